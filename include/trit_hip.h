@@ -422,6 +422,141 @@ int trit_hip_attention_steps_device(const float *q, int qs, const float *const *
                                     const int *tk, int sequences, int d, int heads, int kv_heads, float *out,
                                     void *stream);
 
+/* ---- Serving many sequences ------------------------------------------- */
+
+/* A paged key/value cache of many sequences, held in 8 bits. It has no
+ * counterpart in the reference, whose decoders run one sequence; it stands
+ * beside the session's caches and trit_hip_attention_steps for callers that
+ * decode many requests or beams in their own loop.
+ *
+ * Tokens lie in blocks of 64 of one layer and key head, keys and values
+ * apart. The open block at a sequence's end holds f16 values (a value that
+ * f16 does not hold as a finite one is held as NaN). A block that becomes
+ * full is held as int8 codes and one f32 scale: with a the largest magnitude
+ * of its f16 values, scale = a / 127 (f32), code = round(127 * value / a),
+ * halves to the even one, and the value it stands for code * scale (f32). A
+ * block with a NaN has a NaN scale. What a sequence holds depends on its rows
+ * alone, not on how many came in one call.
+ *
+ * A full block of all layers and heads is a page; sequences that came from
+ * one another share their pages. head_dim 1 to 128 (stored as 64 or 128).
+ *
+ * The handle keeps the sequences' lengths and pages on the host; its calls
+ * queue their device work on `stream` (a hipStream_t; NULL: the calling
+ * thread's stream) without waiting, and run in the order they are made: a
+ * call on another stream than the last one's waits for the device first.
+ * They cannot be captured into a graph. Calls from several threads take
+ * turns. A refused call changes nothing. */
+typedef struct TritHipPagedCache TritHipPagedCache;
+
+/* A cache of `pages` pages and up to `sequences` sequences (at most 2^24 and
+ * 65536). Device memory: layers * kv_heads * (pages * (128 hd + 8) +
+ * sequences * 256 hd) bytes, hd 64 or 128, and sequences * pages * 4. */
+int trit_hip_paged_new(int layers, int kv_heads, int head_dim, int pages, int sequences, TritHipPagedCache **out);
+void trit_hip_paged_free(TritHipPagedCache *cache);
+
+/* n new, empty sequences: their ids in out. */
+int trit_hip_paged_open(TritHipPagedCache *cache, int n, int32_t *out);
+
+/* n new sequences that hold what `sequences` hold (the same one may be named
+ * more than once): pages are shared, open blocks copied. Every layer of a
+ * sequence must hold the same number of tokens, here and in _reorder and
+ * _copy. */
+int trit_hip_paged_fork(TritHipPagedCache *cache, const int32_t *sequences, int n, int32_t *out, void *stream);
+
+/* A beam search's choice: sequence sequences[i] goes on with what parents[i]
+ * held before the call. A parent may be named more than once, need not be
+ * among the sequences, and is copied only where more than one goes on. */
+int trit_hip_paged_reorder(TritHipPagedCache *cache, const int32_t *sequences, const int32_t *parents, int n,
+                           void *stream);
+
+/* n new sequences in `into` (NULL: in `cache`) that hold what `sequences`
+ * hold and share no page with them; what the named ones share among
+ * themselves their copies share. `into` has the cache's layers, kv_heads and
+ * head_dim. */
+int trit_hip_paged_copy(TritHipPagedCache *cache, const int32_t *sequences, int n, TritHipPagedCache *into,
+                        int32_t *out, void *stream);
+
+/* Ends n sequences; pages that no other holds are free again. */
+int trit_hip_paged_close(TritHipPagedCache *cache, const int32_t *sequences, int n);
+
+/* Moves the pages in use to the front of the pool; returns their number. */
+int trit_hip_paged_compact(TritHipPagedCache *cache, void *stream);
+
+/* Another number of pages (no fewer than are in use), in new device memory;
+ * waits for the device. */
+int trit_hip_paged_resize(TritHipPagedCache *cache, int pages, void *stream);
+
+/* Tokens that a sequence holds in `layer`. */
+int trit_hip_paged_length(TritHipPagedCache *cache, int sequence, int layer);
+/* The pool's pages, those in use, and the device bytes of the cache (any may be NULL). */
+int trit_hip_paged_info(TritHipPagedCache *cache, int *pages, int *pages_in_use, int64_t *bytes);
+
+/* Appends rows[i] rows to layer `layer` of sequences[i] (n different ones).
+ * k and v hold the rows one sequence after another, kv_heads * head_dim f32
+ * each; _device: device pointers with strides in floats. Fails when the
+ * pages that become full are not free. */
+int trit_hip_paged_append(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *rows, int n,
+                          const float *k, const float *v);
+int trit_hip_paged_append_device(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *rows,
+                                 int n, const float *k, int64_t k_stride, const float *v, int64_t v_stride,
+                                 void *stream);
+
+/* The values that tokens first[i] .. first[i] + rows[i] - 1 of sequences[i]
+ * stand for, laid out as append takes them. */
+int trit_hip_paged_read(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *first,
+                        const int32_t *rows, int n, float *k, float *v);
+int trit_hip_paged_read_device(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *first,
+                               const int32_t *rows, int n, float *k, int64_t k_stride, float *v, int64_t v_stride,
+                               void *stream);
+
+/* Causal grouped-query attention of the last rows[i] tokens of each
+ * sequences[i] (after their append) over what it holds: row r of a sequence
+ * of `len` tokens sees the first len - rows[i] + r + 1. q holds the rows one
+ * sequence after another, heads * head_dim f32 each (_device: stride q_stride
+ * floats); out is dense, as q's rows. Query head h reads key head h / (heads /
+ * kv_heads). scale: on the scores, 0 for 1/sqrt(head_dim). Sums and softmax
+ * in f32, the queries and probabilities to 24 bits; a NaN in the cache
+ * reaches the rows that see its token (its block's, when that is full).
+ * rows[i] may be 1 (a decode step) up to the tokens held (a prompt). */
+int trit_hip_paged_attention(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *rows, int n,
+                             const float *q, int heads, float scale, float *out);
+int trit_hip_paged_attention_device(TritHipPagedCache *cache, int layer, const int32_t *sequences,
+                                    const int32_t *rows, int n, const float *q, int64_t q_stride, int heads,
+                                    float scale, float *out, void *stream);
+
+/* Cross attention: the keys and values of encoder states (rows that a
+ * decoder layer's key and value projections made of an encoder's output), and
+ * the attention of decoder rows to them -- layers::attention without a mask
+ * (reference src/layers.rs:343-504) for several audios of different lengths
+ * at once, as a batch of beams asks it. `slots` audios of up to max_keys
+ * positions, held as f16 (a value that f16 does not hold as a finite one as
+ * NaN) in layers * slots * kv_heads * max_keys * hd * 4 bytes (hd: head_dim
+ * rounded up to 64 or 128, max_keys to 64). Streams, threads, graphs and
+ * refusals as for the paged cache. */
+typedef struct TritHipCross TritHipCross;
+int trit_hip_cross_new(int layers, int kv_heads, int head_dim, int slots, int max_keys, TritHipCross **out);
+void trit_hip_cross_free(TritHipCross *cross);
+
+/* The states of n different slots in `layer`: keys[i] rows (0 or more) each,
+ * one slot after another, kv_heads * head_dim f32 (_device: device pointers
+ * with strides in floats). They replace what the slots held. */
+int trit_hip_cross_set(TritHipCross *cross, int layer, const int32_t *slots, const int32_t *keys, int n,
+                       const float *k, const float *v);
+int trit_hip_cross_set_device(TritHipCross *cross, int layer, const int32_t *slots, const int32_t *keys, int n,
+                              const float *k, int64_t k_stride, const float *v, int64_t v_stride, void *stream);
+/* Keys that a slot holds. */
+int trit_hip_cross_keys(TritHipCross *cross, int layer, int slot);
+
+/* Attention of rows[i] query rows to every key of slots[i] (a slot may be
+ * named more than once), q, out, heads and scale as
+ * trit_hip_paged_attention. Rows of a slot of no keys are 0. */
+int trit_hip_cross_attention(TritHipCross *cross, int layer, const int32_t *slots, const int32_t *rows, int n,
+                             const float *q, int heads, float scale, float *out);
+int trit_hip_cross_attention_device(TritHipCross *cross, int layer, const int32_t *slots, const int32_t *rows, int n,
+                                    const float *q, int64_t q_stride, int heads, float scale, float *out,
+                                    void *stream);
+
 /* ---- Tokenizer (reference src/text/bpe.rs, src/text/mod.rs) ----------- */
 
 /* Byte-level BPE from a Hugging Face tokenizer.json (Bpe::open / Bpe::parse,

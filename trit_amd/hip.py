@@ -135,6 +135,30 @@ def lib():
             "trit_hip_cleanup_parts": (C.c_int64, [p, C.c_char_p, C.c_size_t, i, p, C.c_size_t]),
             "trit_hip_attention_steps": (i, [p, i, p, p, p, i, i, i, i, p]),
             "trit_hip_attention_steps_device": (i, [p, i, p, p, p, i, i, i, i, p, p]),
+            "trit_hip_paged_new": (i, [i, i, i, i, i, pp]),
+            "trit_hip_paged_free": (None, [p]),
+            "trit_hip_paged_open": (i, [p, i, p]),
+            "trit_hip_paged_fork": (i, [p, p, i, p, p]),
+            "trit_hip_paged_reorder": (i, [p, p, p, i, p]),
+            "trit_hip_paged_copy": (i, [p, p, i, p, p, p]),
+            "trit_hip_paged_close": (i, [p, p, i]),
+            "trit_hip_paged_compact": (i, [p, p]),
+            "trit_hip_paged_resize": (i, [p, i, p]),
+            "trit_hip_paged_length": (i, [p, i, i]),
+            "trit_hip_paged_info": (i, [p, C.POINTER(i), C.POINTER(i), C.POINTER(C.c_int64)]),
+            "trit_hip_paged_append": (i, [p, i, p, p, i, p, p]),
+            "trit_hip_paged_append_device": (i, [p, i, p, p, i, p, C.c_int64, p, C.c_int64, p]),
+            "trit_hip_paged_read": (i, [p, i, p, p, p, i, p, p]),
+            "trit_hip_paged_read_device": (i, [p, i, p, p, p, i, p, C.c_int64, p, C.c_int64, p]),
+            "trit_hip_paged_attention": (i, [p, i, p, p, i, p, i, f, p]),
+            "trit_hip_paged_attention_device": (i, [p, i, p, p, i, p, C.c_int64, i, f, p, p]),
+            "trit_hip_cross_new": (i, [i, i, i, i, i, pp]),
+            "trit_hip_cross_free": (None, [p]),
+            "trit_hip_cross_set": (i, [p, i, p, p, i, p, p]),
+            "trit_hip_cross_set_device": (i, [p, i, p, p, i, p, C.c_int64, p, C.c_int64, p]),
+            "trit_hip_cross_keys": (i, [p, i, i]),
+            "trit_hip_cross_attention": (i, [p, i, p, p, i, p, i, f, p]),
+            "trit_hip_cross_attention_device": (i, [p, i, p, p, i, p, C.c_int64, i, f, p, p]),
         }
         for name, (res, args) in sig.items():
             if not hasattr(L, name):
@@ -710,6 +734,206 @@ class Session:
     def free(self):
         if self.h:
             lib().trit_hip_session_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _ids(values):
+    """Sequence ids, slots or row counts as the C calls read them (an int32 array as it is)."""
+    if isinstance(values, np.ndarray) and values.dtype == np.int32 and values.flags.c_contiguous and values.ndim == 1:
+        return values
+    return np.ascontiguousarray(np.asarray(values, dtype=np.int32).reshape(-1))
+
+
+def _counts(ids, counts, what):
+    counts = _ids(counts)
+    if counts.size != ids.size:
+        raise TritError(f"{what}: {ids.size} ids and {counts.size} counts")
+    return counts
+
+
+class PagedCache:
+    """A paged 8-bit key/value cache of many sequences (trit_hip_paged_new).
+
+    Methods without `_device` take and return host arrays and wait; those with
+    it take device addresses (ints) and row strides in floats, and queue their
+    work on `stream` (None: the calling thread's stream), as do fork, reorder,
+    copy and compact. Sequences are named by the ids that open, fork and copy
+    return."""
+
+    BLOCK = 64
+
+    def __init__(self, layers, kv_heads, head_dim, pages, sequences):
+        self.h = None
+        self.layers, self.kv_heads, self.head_dim = layers, kv_heads, head_dim
+        out = C.c_void_p()
+        check(lib().trit_hip_paged_new(layers, kv_heads, head_dim, pages, sequences, C.byref(out)))
+        self.h = out
+
+    def open(self, n=1):
+        out = np.empty(max(n, 0), np.int32)
+        check(lib().trit_hip_paged_open(self.h, n, ptr(out)))
+        return out
+
+    def fork(self, sequences, stream=None):
+        ids = _ids(sequences)
+        out = np.empty(ids.size, np.int32)
+        check(lib().trit_hip_paged_fork(self.h, ptr(ids), ids.size, ptr(out), stream))
+        return out
+
+    def reorder(self, sequences, parents, stream=None):
+        ids = _ids(sequences)
+        parents = _counts(ids, parents, "paged reorder")
+        check(lib().trit_hip_paged_reorder(self.h, ptr(ids), ptr(parents), ids.size, stream))
+
+    def copy(self, sequences, into=None, stream=None):
+        ids = _ids(sequences)
+        out = np.empty(ids.size, np.int32)
+        check(lib().trit_hip_paged_copy(self.h, ptr(ids), ids.size, into.h if into is not None else None, ptr(out),
+                                        stream))
+        return out
+
+    def close(self, sequences):
+        ids = _ids(sequences)
+        check(lib().trit_hip_paged_close(self.h, ptr(ids), ids.size))
+
+    def compact(self, stream=None):
+        return check(lib().trit_hip_paged_compact(self.h, stream))
+
+    def resize(self, pages, stream=None):
+        check(lib().trit_hip_paged_resize(self.h, pages, stream))
+
+    def length(self, sequence, layer=0):
+        return check(lib().trit_hip_paged_length(self.h, int(sequence), layer))
+
+    def info(self):
+        pages, used, nbytes = C.c_int(), C.c_int(), C.c_int64()
+        check(lib().trit_hip_paged_info(self.h, C.byref(pages), C.byref(used), C.byref(nbytes)))
+        return {"pages": pages.value, "used": used.value, "bytes": nbytes.value}
+
+    def _host_rows(self, rows, total, width, what):
+        rows = np.ascontiguousarray(rows, np.float32)
+        if rows.size != total * width:
+            raise TritError(f"{what}: {rows.size} values where {total} rows of {width} are needed")
+        return rows
+
+    def append(self, layer, sequences, rows, k, v):
+        """rows[i] rows of keys and values (kv_heads * head_dim each) to sequences[i]."""
+        ids = _ids(sequences)
+        rows = _counts(ids, rows, "paged append")
+        total, width = int(rows.sum()), self.kv_heads * self.head_dim
+        k = self._host_rows(k, total, width, "paged append")
+        v = self._host_rows(v, total, width, "paged append")
+        check(lib().trit_hip_paged_append(self.h, layer, ptr(ids), ptr(rows), ids.size, ptr(k), ptr(v)))
+
+    def append_device(self, layer, sequences, rows, k, k_stride, v, v_stride, stream=None):
+        ids = _ids(sequences)
+        rows = _counts(ids, rows, "paged append")
+        check(lib().trit_hip_paged_append_device(self.h, layer, ptr(ids), ptr(rows), ids.size, k, k_stride, v, v_stride,
+                                                 stream))
+
+    def read(self, layer, sequences, first, rows):
+        """The values that rows[i] tokens from first[i] on of sequences[i] stand for: keys and values."""
+        ids = _ids(sequences)
+        first, rows = _counts(ids, first, "paged read"), _counts(ids, rows, "paged read")
+        shape = (max(int(rows.sum()), 0), self.kv_heads * self.head_dim)
+        k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
+        check(lib().trit_hip_paged_read(self.h, layer, ptr(ids), ptr(first), ptr(rows), ids.size, ptr(k), ptr(v)))
+        return k, v
+
+    def read_device(self, layer, sequences, first, rows, k, k_stride, v, v_stride, stream=None):
+        ids = _ids(sequences)
+        first, rows = _counts(ids, first, "paged read"), _counts(ids, rows, "paged read")
+        check(lib().trit_hip_paged_read_device(self.h, layer, ptr(ids), ptr(first), ptr(rows), ids.size, k, k_stride, v,
+                                               v_stride, stream))
+
+    def attention(self, layer, sequences, rows, q, heads, scale=0.0):
+        """Causal attention of the last rows[i] tokens of sequences[i]: q and the result heads * head_dim a row."""
+        ids = _ids(sequences)
+        rows = _counts(ids, rows, "paged attention")
+        total, width = int(rows.sum()), heads * self.head_dim
+        q = self._host_rows(q, total, width, "paged attention")
+        out = np.empty((max(total, 0), max(width, 0)), np.float32)
+        check(lib().trit_hip_paged_attention(self.h, layer, ptr(ids), ptr(rows), ids.size, ptr(q), heads, scale,
+                                             ptr(out)))
+        return out
+
+    def attention_device(self, layer, sequences, rows, q, q_stride, heads, out, scale=0.0, stream=None):
+        ids = _ids(sequences)
+        rows = _counts(ids, rows, "paged attention")
+        check(lib().trit_hip_paged_attention_device(self.h, layer, ptr(ids), ptr(rows), ids.size, q, q_stride, heads,
+                                                    scale, out, stream))
+
+    def free(self):
+        if self.h:
+            lib().trit_hip_paged_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class CrossStates:
+    """The keys and values of several audios' encoder states, and the
+    attention of decoder rows to them (trit_hip_cross_new). Host and device
+    methods as PagedCache's."""
+
+    def __init__(self, layers, kv_heads, head_dim, slots, max_keys):
+        self.h = None
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        out = C.c_void_p()
+        check(lib().trit_hip_cross_new(layers, kv_heads, head_dim, slots, max_keys, C.byref(out)))
+        self.h = out
+
+    def set(self, layer, slots, keys, k, v):
+        """keys[i] rows of keys and values (kv_heads * head_dim each) as the states of slots[i]."""
+        slots = _ids(slots)
+        keys = _counts(slots, keys, "cross set")
+        total, width = int(keys.sum()), self.kv_heads * self.head_dim
+        k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
+        if k.size != total * width or v.size != total * width:
+            raise TritError(f"cross set: {k.size} and {v.size} values where {total} rows of {width} are needed")
+        check(lib().trit_hip_cross_set(self.h, layer, ptr(slots), ptr(keys), slots.size, ptr(k), ptr(v)))
+
+    def set_device(self, layer, slots, keys, k, k_stride, v, v_stride, stream=None):
+        slots = _ids(slots)
+        keys = _counts(slots, keys, "cross set")
+        check(lib().trit_hip_cross_set_device(self.h, layer, ptr(slots), ptr(keys), slots.size, k, k_stride, v, v_stride,
+                                              stream))
+
+    def keys(self, slot, layer=0):
+        return check(lib().trit_hip_cross_keys(self.h, layer, int(slot)))
+
+    def attention(self, layer, slots, rows, q, heads, scale=0.0):
+        """Attention of rows[i] rows to every key of slots[i]: q and the result heads * head_dim a row."""
+        slots = _ids(slots)
+        rows = _counts(slots, rows, "cross attention")
+        total, width = int(rows.sum()), heads * self.head_dim
+        q = np.ascontiguousarray(q, np.float32)
+        if q.size != total * width:
+            raise TritError(f"cross attention: {q.size} values where {total} rows of {width} are needed")
+        out = np.empty((max(total, 0), max(width, 0)), np.float32)
+        check(lib().trit_hip_cross_attention(self.h, layer, ptr(slots), ptr(rows), slots.size, ptr(q), heads, scale,
+                                             ptr(out)))
+        return out
+
+    def attention_device(self, layer, slots, rows, q, q_stride, heads, out, scale=0.0, stream=None):
+        slots = _ids(slots)
+        rows = _counts(slots, rows, "cross attention")
+        check(lib().trit_hip_cross_attention_device(self.h, layer, ptr(slots), ptr(rows), slots.size, q, q_stride, heads,
+                                                    scale, out, stream))
+
+    def free(self):
+        if self.h:
+            lib().trit_hip_cross_free(self.h)
             self.h = None
 
     def __del__(self):
