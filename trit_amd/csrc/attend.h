@@ -42,7 +42,17 @@ struct AttendSeq {
     int len;    // keys
     int rows;   // query rows
     int first;  // its first row in q and out
-    int start;  // its first item of the launch (set by attend())
+    // Set by attend(): its first item of the launch, its first group of items
+    // that are joined, the items its keys are split into.
+    int start, group, chunks;
+};
+
+// Device memory of a handle for keys that are split over workgroups: each
+// one's sums, and a counter for each group of them (0 between launches).
+struct AttendScratch {
+    DeviceMemory memory;
+    // For heads of hdp (64 or 128) values; clears the counters on `s`.
+    void make(int hdp, hipStream_t s);
 };
 
 struct AttendArgs {
@@ -61,12 +71,17 @@ struct AttendArgs {
     // blocks), or `blocks` of them (states).
     const _Float16* f16 = nullptr;
     int blocks = 1;
-    // Set by attend().
+    // Set by attend(): the scratch's parts, and the blocks of a chunk.
+    float* sums = nullptr;
+    uint64_t* tops = nullptr;
+    int* counters = nullptr;
+    int chunk = 0;
     int n = 0;
     AttendSeq s[CALL_SEQS];
 };
 
-// `seqs`: n of them; a.place .. first set. Queued on `s`.
-void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, hipStream_t s);
+// `seqs`: place .. first set. Queued on `s`, where no other call with the same
+// scratch may overlap.
+void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, AttendScratch& scratch, hipStream_t s);
 
 }  // namespace trit

@@ -1,6 +1,6 @@
 // Attention of a few or many query rows to int8 blocks (a paged cache's full
 // ones) and f16 blocks (its open ones, or an encoder's states).
-#include <algorithm>
+#include <climits>
 
 #include "attend.h"
 #include "device.h"
@@ -351,14 +351,34 @@ __device__ __forceinline__ void f16_block(const _Float16* block, int tokens, con
     }
 }
 
-// Block (item): sequence, key head g and a tile of 16 columns (query row r,
-// head g * group + c of it: column r * group + c); its four waves take the
-// key blocks in turn and join their sums in shared memory.
+__global__ void clear_kernel(int* p, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
+}
+
+// Words that other workgroups of the launch read: to and from memory past the
+// caches that a reader on another XCD does not share.
+__device__ __forceinline__ void put(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put(uint64_t* p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get(const float* p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Block (item): sequence, key head g, a tile of 16 columns (query row r, head
+// g * group + c of it: column r * group + c) and a chunk of its key blocks.
+// The four waves take the chunk's blocks in turn and join their sums in shared
+// memory. Of the workgroups of a tile's chunks the last to end joins theirs,
+// in the chunks' order.
 template <int HDP, bool PAGED>
 __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
     constexpr int NT = HDP / 16;
     __shared__ float top[WAVES][16], sum[WAVES][16];
     __shared__ float part[WAVES][16][HDP];
+    __shared__ bool arrived;
     const int t = threadIdx.x, w = t / WAVE, lane = t % WAVE, col = lane % 16, lq = lane / 16;
     // The last sequence whose items start at or before this one.
     int si = 0;
@@ -367,7 +387,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
         si += __popcll(__ballot(i + lane < a.n && a.s[i + lane].start <= (int)blockIdx.x));
     const AttendSeq seq = a.s[si - 1];
     const int item = (int)blockIdx.x - seq.start;
-    const int g = item % a.kv_heads, tile = item / a.kv_heads;
+    const int g = item % a.kv_heads, chunk = item / a.kv_heads % seq.chunks, tile = item / a.kv_heads / seq.chunks;
     const int columns = seq.rows * a.group;
     const int c = tile * 16 + col, row = c / a.group;
     const int head = g * a.group + c % a.group;
@@ -377,7 +397,8 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
     const int last = (tile * 16 + 15 < columns ? tile * 16 + 15 : columns - 1) / a.group;
     const int most = PAGED ? ahead + last : ahead, least = PAGED ? ahead + tile * 16 / a.group : ahead;
     const int seen = c < columns ? (PAGED ? ahead + row : ahead) : 0;
-    const int end = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+    const int b0 = chunk * a.chunk;
+    const int all = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS, end = all < b0 + a.chunk ? all : b0 + a.chunk;
 
     Running<HDP> run;
     run.clear();
@@ -386,7 +407,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
         const int* table = a.table + (size_t)seq.place * a.table_stride;
         Digits<HDP> qd;
         query_digits<HDP>(q, a.hd, a.scale, qd);
-        int b = w;
+        int b = b0 + w;
         for (; b < end && b < full; b += WAVES) {
             const size_t at = (size_t)table[b] * a.kv_heads + g;
             const uint8_t* block = a.codes + at * (2 * BLOCK_TOKENS * HDP);
@@ -406,7 +427,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
         Pairs<HDP> qp;
         query_pairs<HDP>(q, a.hd, a.scale, qp);
         const _Float16* states = a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * (2 * BLOCK_TOKENS * HDP);
-        for (int b = w; b < end; b += WAVES)
+        for (int b = b0 + w; b < end; b += WAVES)
             f16_block<HDP, false>(states + (size_t)b * (2 * BLOCK_TOKENS * HDP), seq.len - b * BLOCK_TOKENS, qp,
                                   seq.len - b * BLOCK_TOKENS, run);
     }
@@ -420,13 +441,14 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) part[w][col][16 * n + 4 * lq + r] = run.acc[n][r];
     __syncthreads();
-    for (int i = t; i < 16 * HDP; i += WAVES * WAVE) {
-        const int cc = i / HDP, e = i % HDP;
-        if (tile * 16 + cc >= columns || e >= a.hd) continue;
-        float m = top[0][cc];
+    const int cols = min(columns - tile * 16, 16);
+    // The sums of the waves' parts, relative to their largest score m.
+    auto joined = [&](int cc, int e, float& m, float& l) {
+        m = top[0][cc];
 #pragma unroll
         for (int v = 1; v < WAVES; ++v) m = __builtin_fmaxf(m, top[v][cc]);
-        float o = 0.0f, l = 0.0f;
+        float o = 0.0f;
+        l = 0.0f;
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
             // A wave that saw no key has sums of 0; NaN sums stay NaN.
@@ -434,34 +456,133 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
             o = __builtin_fmaf(part[v][cc][e], f, o);
             l = __builtin_fmaf(sum[v][cc], f, l);
         }
+        return o;
+    };
+    auto store = [&](int cc, int e, float o, float l) {
         const int rr = (tile * 16 + cc) / a.group, hh = g * a.group + (tile * 16 + cc) % a.group;
         // No key at all: 0.
-        a.out[((size_t)(seq.first + rr) * a.kv_heads * a.group + hh) * a.hd + e] = l == 0.0f ? 0.0f : o / l;
+        if (e < a.hd) a.out[((size_t)(seq.first + rr) * a.kv_heads * a.group + hh) * a.hd + e] = l == 0.0f ? 0.0f : o / l;
+    };
+    if (seq.chunks == 1) {
+        for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
+            float m, l;
+            const float o = joined(i / HDP, i % HDP, m, l);
+            store(i / HDP, i % HDP, o, l);
+        }
+        return;
+    }
+    for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
+        const int cc = i / HDP, e = i % HDP;
+        float m, l;
+        const float o = joined(cc, e, m, l);
+        const size_t at = (size_t)blockIdx.x * 16 + cc;
+        put(a.sums + at * HDP + e, o);
+        if (e == 0) put(a.tops + at, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(m));
+    }
+    // Every store of the workgroup is in memory before its arrival is counted.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* counter = a.counters + seq.group + tile * a.kv_heads + g;
+    if (t == 0) {
+        const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        arrived = before + 1 == seq.chunks;
+        if (before + 1 == seq.chunks) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!arrived) return;
+    // Chunk v's item; wave w joins the chunks w, w + 4, .. of each column, lane l their elements 2 l, 2 l + 1.
+    const size_t first = (size_t)seq.start + (size_t)tile * seq.chunks * a.kv_heads + g;
+    for (int cc = 0; cc < cols; ++cc) {
+        float m = -INFINITY, l = 0.0f;
+        float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+        for (int v = w; v < seq.chunks; v += WAVES) {
+            const size_t at = (first + (size_t)v * a.kv_heads) * 16 + cc;
+            const float2 ml = get((const float*)(a.tops + at));
+            const float2 x = 2 * lane < HDP ? get(a.sums + at * HDP + 2 * lane) : make_float2(0.0f, 0.0f);
+            const float mn = __builtin_fmaxf(m, ml.x);
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float h = ml.x == mn ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+            l = __builtin_fmaf(ml.y, h, l * f);
+            o.x = __builtin_fmaf(x.x, h, o.x * f);
+            o.y = __builtin_fmaf(x.y, h, o.y * f);
+            m = mn;
+        }
+        if (lane == 0) {
+            top[w][cc] = m;
+            sum[w][cc] = l;
+        }
+        if (2 * lane < HDP) {
+            part[w][cc][2 * lane] = o.x;
+            part[w][cc][2 * lane + 1] = o.y;
+        }
+    }
+    __syncthreads();
+    for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
+        float m, l;
+        const float o = joined(i / HDP, i % HDP, m, l);
+        store(i / HDP, i % HDP, o, l);
     }
 }
 
 }  // namespace
 
-// Items of one launch (a grid holds fewer than 2^32 threads).
+// Items of one launch (a grid holds fewer than 2^32 threads), and the most
+// where keys are split: what the scratch holds.
 constexpr long long MOST_ITEMS = 1 << 23;
+constexpr long long SPLIT_ITEMS = 1024;
 
-void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, hipStream_t s) {
+void AttendScratch::make(int hdp, hipStream_t s) {
+    memory.alloc(SPLIT_ITEMS * (16 * ((size_t)hdp * 4 + 8) + 4));
+    // The counters are the last part.
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, (int*)((char*)memory.ptr + memory.bytes) - SPLIT_ITEMS,
+                       (int)SPLIT_ITEMS);
+    TRIT_HIP(hipGetLastError());
+}
+
+void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, AttendScratch& scratch, hipStream_t s) {
+    const int hdp = a.hd <= 64 ? 64 : 128;
+    a.sums = scratch.memory.as<float>();
+    a.tops = (uint64_t*)(a.sums + SPLIT_ITEMS * 16 * hdp);
+    a.counters = (int*)(a.tops + SPLIT_ITEMS * 16);
+    const auto tiles = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 15) / 16; };
+    const auto blocks = [](const AttendSeq& q) { return (q.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS; };
     for (size_t from = 0; from < seqs.size();) {
-        long long items = 0;
-        a.n = 0;
-        for (; from < seqs.size() && a.n < CALL_SEQS; ++from) {
-            AttendSeq one = seqs[from];
-            if (one.rows == 0) continue;
-            const long long tiles = ((long long)one.rows * a.group + 15) / 16;
-            if (a.n && items + tiles * a.kv_heads > MOST_ITEMS) break;
-            if (tiles * a.kv_heads > MOST_ITEMS) fail("attention: more query rows than one launch takes");
-            one.start = (int)items;
-            items += tiles * a.kv_heads;
-            a.s[a.n++] = one;
+        // The launch's sequences, and its work in blocks of keys.
+        long long whole = 0, work = 0;
+        size_t to = from;
+        for (a.n = 0; to < seqs.size() && a.n < CALL_SEQS; ++to) {
+            if (seqs[to].rows == 0) continue;
+            const long long items = tiles(seqs[to]) * a.kv_heads;
+            if (items > MOST_ITEMS) fail("attention: more query rows than one launch takes");
+            if (a.n && whole + items > MOST_ITEMS) break;
+            whole += items;
+            work += items * blocks(seqs[to]);
+            a.s[a.n++] = seqs[to];
         }
+        from = to;
         if (!a.n) return;
+        // Chunks of as few blocks as keep the items within the scratch, a multiple of what the waves take at once.
+        long long items = whole;
+        a.chunk = INT_MAX / 2;
+        if (whole < SPLIT_ITEMS) {
+            const long long room = SPLIT_ITEMS - whole;
+            a.chunk = (int)((work + room - 1) / room + WAVES - 1) / WAVES * WAVES;
+            if (a.chunk < WAVES) a.chunk = WAVES;
+        }
+        items = 0;
+        int groups = 0;
+        for (int i = 0; i < a.n; ++i) {
+            AttendSeq& q = a.s[i];
+            const int nb = blocks(q);
+            q.chunks = nb <= a.chunk ? 1 : (nb + a.chunk - 1) / a.chunk;
+            q.start = (int)items;
+            q.group = groups;
+            items += tiles(q) * a.kv_heads * q.chunks;
+            if (q.chunks > 1) groups += (int)tiles(q) * a.kv_heads;
+        }
         const dim3 grid((unsigned)items), block(WAVES * WAVE);
-        if (a.hd <= 64) {
+        if (hdp == 64) {
             if (paged)
                 hipLaunchKernelGGL((attend_kernel<64, true>), grid, block, 0, s, a);
             else

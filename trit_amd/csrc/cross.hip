@@ -54,6 +54,7 @@ using namespace trit;
 struct TritHipCross {
     int device, layers, kv_heads, hd, hdp, slots, max_keys, blocks;
     DeviceMemory states;
+    AttendScratch scratch;
     std::vector<int> keys;  // by layer and slot; -1: never set
     // The stream of the last call; one on another waits for the device first.
     hipStream_t last = nullptr;
@@ -129,6 +130,7 @@ int trit_hip_cross_new(int layers, int kv_heads, int head_dim, int slots, int ma
         c->blocks = (max_keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
         c->keys.assign((size_t)layers * slots, -1);
         c->states.alloc((size_t)layers * c->layer_values() * 2);
+        c->scratch.make(c->hdp, c->enter(nullptr));
         *out = c.release();
         return 0;
     });
@@ -228,7 +230,7 @@ int trit_hip_cross_attention_device(TritHipCross* cross, int layer, const int32_
             if (keys < 0)
                 fail("cross attention: slot " + std::to_string(slots[i]) + " of layer " + std::to_string(layer) +
                      " was never set");
-            seqs.push_back({slots[i], keys, rows[i], first, 0});
+            seqs.push_back({slots[i], keys, rows[i], first, 0, 0, 0});
             first += rows[i];
         }
         const hipStream_t s = cross->enter(stream_);
@@ -242,7 +244,7 @@ int trit_hip_cross_attention_device(TritHipCross* cross, int layer, const int32_
         a.hd = cross->hd;
         a.f16 = cross->states.as<_Float16>() + (size_t)layer * cross->layer_values();
         a.blocks = cross->blocks;
-        attend(a, seqs, false, s);
+        attend(a, seqs, false, cross->scratch, s);
         return 0;
     });
 }

@@ -239,6 +239,7 @@ struct TritHipPagedCache {
     int device, layers, kv_heads, hd, hdp;
     PageBook book;
     DeviceMemory codes, scales, open, table;
+    AttendScratch scratch;
     // The stream of the last call. A call on another one waits for the device
     // first: the books run ahead of it, and a page freed by one call may be
     // the one that the next call writes.
@@ -367,6 +368,7 @@ int trit_hip_paged_new(int layers, int kv_heads, int head_dim, int pages, int se
         hipLaunchKernelGGL(clear_kernel, dim3(1024), dim3(THREADS), 0, c->enter(nullptr), c->open.as<uint4>(),
                            c->open.bytes / 16);
         TRIT_HIP(hipGetLastError());
+        c->scratch.make(c->hdp, c->last);
         *out = c.release();
         return 0;
     });
@@ -653,7 +655,7 @@ int trit_hip_paged_attention_device(TritHipPagedCache* cache, int layer, const i
             if (rows[i] > len)
                 fail("paged attention: " + std::to_string(rows[i]) + " query rows of sequence " +
                      std::to_string(sequences[i]) + ", which holds " + std::to_string(len) + " tokens");
-            seqs.push_back({cache->book.row(sequences[i]), len, rows[i], first, 0});
+            seqs.push_back({cache->book.row(sequences[i]), len, rows[i], first, 0, 0, 0});
             first += rows[i];
         }
         const hipStream_t s = cache->enter(stream_);
@@ -671,7 +673,7 @@ int trit_hip_paged_attention_device(TritHipPagedCache* cache, int layer, const i
         a.table = p.table;
         a.table_stride = p.pages;
         a.f16 = p.open;
-        attend(a, seqs, true, s);
+        attend(a, seqs, true, cache->scratch, s);
         return 0;
     });
 }
