@@ -76,6 +76,7 @@ struct AttendArgs {
     uint64_t* tops = nullptr;
     int* counters = nullptr;
     int chunk = 0;
+    bool aligned = false;  // 16-byte loads of the queries
     int n = 0;
     AttendSeq s[CALL_SEQS];
 };

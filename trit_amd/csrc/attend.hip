@@ -67,145 +67,149 @@ struct Running {
 };
 
 // Scores u * f (f >= 0 or NaN) of a block to probabilities of that block
-// alone, p = 2^(u f - max) <= 1, in place; then the running maximum takes the
-// block's. `before` scales what was summed, `now` the block's products: a
-// block's probabilities are fixed-point values or f16 pairs relative to its
-// own maximum, so that a long tail of small ones next to one large one far
-// away keeps its digits. seen: the columns' keys from this block on; values
-// from there on do not count, whatever they hold.
-// Returns whether the column sees any of the block.
-template <bool MASK>
-__device__ __forceinline__ bool block_softmax(float (&u)[16], float f, int seen, float& m, float& l, float& before,
-                                              float& now) {
+// alone, p = 2^((u - max) f) <= 1, in place; then the running sums take the
+// block's largest score as theirs. Returned: what scales the block's products
+// (0 where the column sees none of it). A block's probabilities become
+// fixed-point values or f16 pairs relative to its own maximum, so that a long
+// tail of small ones next to one large one far away keeps its digits. mask
+// (the same for the wave): `seen` of the block's tokens count, whatever the
+// others hold.
+template <int HDP>
+__device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mask, int seen, Running<HDP>& run) {
     const int lq = (threadIdx.x % WAVE) / 16;
-    float top = -INFINITY;
+    if (mask) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (MASK && 16 * (i / 4) + 4 * lq + i % 4 >= seen) u[i] = -INFINITY;
-        top = __builtin_fmaxf(top, u[i]);
+        for (int i = 0; i < 16; ++i)
+            if (16 * (i / 4) + 4 * lq + i % 4 >= seen) u[i] = -INFINITY;
     }
+    float top = u[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i]);
     top = column_max(top);
-    const bool any = !MASK || top > -INFINITY;
+    const bool any = top > -INFINITY;
     const float mb = any ? top * f : -INFINITY;
+    // The difference first: never above 0, whatever the scores' size.
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i] = __builtin_amdgcn_exp2f((u[i] - top) * f);
+    if (mask) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (16 * (i / 4) + 4 * lq + i % 4 >= seen) u[i] = 0.0f;
+    }
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        // The difference first: never above 0, whatever the scores' size.
-        const float p = __builtin_amdgcn_exp2f((u[i] - top) * f);
-        u[i] = MASK && 16 * (i / 4) + 4 * lq + i % 4 >= seen ? 0.0f : p;
-        sum += u[i];
+    for (int i = 0; i < 16; ++i) sum += u[i];
+    const float mn = __builtin_fmaxf(run.m, mb);
+    const float before = mn == run.m ? 1.0f : __builtin_amdgcn_exp2f(run.m - mn);
+    const float now = any ? __builtin_amdgcn_exp2f(mb - mn) : 0.0f;
+    run.m = mn;
+    run.l = __builtin_fmaf(now, sum, run.l * before);
+    if (__any(before != 1.0f)) {
+#pragma unroll
+        for (int n = 0; n < HDP / 16; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) run.acc[n][r] *= before;
     }
-    const float mn = __builtin_fmaxf(m, mb);
-    before = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    now = any ? __builtin_amdgcn_exp2f(mb - mn) : 0.0f;
-    m = mn;
-    l = __builtin_fmaf(now, sum, l * before);
-    return any;
+    return now;
 }
 
-// The columns' queries as fixed point: x = round(q * FIXED / max|q|), three
-// digits, and the step max|q| / FIXED (times scale and log2 e).
-template <int HDP>
-struct Digits {
-    v4i d[3][HDP / 64];
-    float step;
+// The 16 columns' queries in shared memory, each part in its operand order (a
+// wave's lane reads 16 bytes at 16 * lane of each 1 KB):
+//  digits: fixed point round(q * FIXED / max|q|), three digits;
+//  pairs: f16 values hi + lo of q * PAIR / max|q|;
+//  top: max|q|, NaN for a query with a NaN or an infinity.
+template <int HDP, bool DIGITS>
+struct Queries {
+    __align__(16) int8_t digits[3][DIGITS ? 16 * HDP : 16];
+    __align__(16) _Float16 pairs[2][16 * HDP];
+    float top[16];
 };
 
-// 16 or 8 consecutive values of a query, 0 past head_dim or for no query.
-template <int N>
-__device__ __forceinline__ void load_query(const float* q, int e, int hd, float scale, float (&v)[N]) {
+// Thread 16 c + i of the workgroup takes HDP / 16 consecutive values of column
+// c; q: its values, or any readable address with valid false. (Loads under a
+// condition each would wait for each: 13 us of a 15 us launch.)
+template <int HDP, bool DIGITS>
+__device__ __forceinline__ void load_queries(const float* q, bool valid, bool aligned, int hd, float scale,
+                                             float (&v)[HDP / 16]) {
+    constexpr int E = HDP / 16;
+    const int e0 = threadIdx.x % 16 * E;
+    if (aligned) {  // head_dim a multiple of 4
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = q && e + i < hd ? q[e + i] * scale : 0.0f;
-}
-
-template <int HDP>
-__device__ __forceinline__ void query_digits(const float* q, int hd, float scale, Digits<HDP>& out) {
-    const int lq = (threadIdx.x % WAVE) / 16;
-    float v[HDP / 64][16], top = 0.0f;
-    bool bad = false;
-#pragma unroll
-    for (int ks = 0; ks < HDP / 64; ++ks) {
-        load_query(q, 64 * ks + 16 * lq, hd, scale, v[ks]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            top = __builtin_fmaxf(top, __builtin_fabsf(v[ks][i]));
-            bad |= v[ks][i] != v[ks][i];
+        for (int i = 0; i < E; i += 4) {
+            const float4 x = gload_f4(q + (e0 + i < hd ? e0 + i : 0));
+            v[i] = x.x;
+            v[i + 1] = x.y;
+            v[i + 2] = x.z;
+            v[i + 3] = x.w;
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = *gmem(q + (e0 + i < hd ? e0 + i : 0));
     }
-    // A query that holds a NaN has NaN scores (a maximum passes over it).
-    top = column_max(bad ? INFINITY : top);
-    // Queries below 1e-30 have scores that differ by nothing; an infinite
-    // one has no digits and NaN scores.
-    const float inv = FIXED / __builtin_fmaxf(top, 1e-30f);
-    out.step = top < INFINITY ? __builtin_fmaxf(top, 1e-30f) * (1.0f / FIXED) * LOG2E : NAN;
 #pragma unroll
-    for (int ks = 0; ks < HDP / 64; ++ks)
+    for (int i = 0; i < E; ++i) v[i] = valid && e0 + i < hd ? v[i] * scale : 0.0f;
+}
+template <int HDP, bool DIGITS>
+__device__ __forceinline__ void put_queries(const float (&v)[HDP / 16], Queries<HDP, DIGITS>& out) {
+    constexpr int E = HDP / 16;
+    const int col = threadIdx.x / 16, e0 = threadIdx.x % 16 * E;
+    float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < E; ++i) top = v[i] == v[i] ? __builtin_fmaxf(top, __builtin_fabsf(v[i])) : INFINITY;
+    top = __builtin_fmaxf(top, dpp<DPP_XOR1>(top));
+    top = __builtin_fmaxf(top, dpp<DPP_XOR2>(top));
+    top = __builtin_fmaxf(top, dpp<DPP_HALF_MIRROR>(top));
+    top = __builtin_fmaxf(top, dpp<DPP_MIRROR>(top));
+    const bool finite = top < INFINITY;
+    // Queries below 1e-30 have scores that differ by nothing.
+    top = __builtin_fmaxf(top, 1e-30f);
+    if (threadIdx.x % 16 == 0) out.top[col] = finite ? top : NAN;
+    if (DIGITS) {
+        const float inv = FIXED / top;
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
             uint32_t x[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float s = __builtin_rintf(v[ks][4 * i + r] * inv);
-                x[r] = (uint32_t)(int)__builtin_fminf(__builtin_fmaxf(s, -FIXED), FIXED);
-            }
-            int d0, d1, d2;
-            digits4(x[0], x[1], x[2], x[3], d0, d1, d2);
-            out.d[0][ks][i] = d0;
-            out.d[1][ks][i] = d1;
-            out.d[2][ks][i] = d2;
-        }
-}
-
-// The columns' queries as pairs of f16 values hi + lo, scaled to a largest
-// magnitude of PAIR; step as above.
-template <int HDP>
-struct Pairs {
-    v8h hi[HDP / 32], lo[HDP / 32];
-    float step;
-};
-template <int HDP>
-__device__ __forceinline__ void query_pairs(const float* q, int hd, float scale, Pairs<HDP>& out) {
-    const int lq = (threadIdx.x % WAVE) / 16;
-    float v[HDP / 32][8], top = 0.0f;
-    bool bad = false;
+            for (int r = 0; r < 4; ++r) x[r] = finite ? (uint32_t)(int)__builtin_rintf(v[i + r] * inv) : 0u;
+            int d[3];
+            digits4(x[0], x[1], x[2], x[3], d[0], d[1], d[2]);
+            const int e = e0 + i, at = e / 64 * 1024 + (e % 64 / 16 * 16 + col) * 16 + e % 16;
 #pragma unroll
-    for (int ks = 0; ks < HDP / 32; ++ks) {
-        load_query(q, 32 * ks + 8 * lq, hd, scale, v[ks]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            top = __builtin_fmaxf(top, __builtin_fabsf(v[ks][i]));
-            bad |= v[ks][i] != v[ks][i];
+            for (int j = 0; j < 3; ++j) *(int*)(out.digits[j] + at) = d[j];
         }
     }
-    top = column_max(bad ? INFINITY : top);
-    const float inv = PAIR / __builtin_fmaxf(top, 1e-30f);
-    out.step = top < INFINITY ? __builtin_fmaxf(top, 1e-30f) * (1.0f / PAIR) * LOG2E : NAN;
+    const float inv = PAIR / top;
 #pragma unroll
-    for (int ks = 0; ks < HDP / 32; ++ks)
+    for (int i = 0; i < E; i += 4) {
+        const int e = e0 + i, at = e / 32 * 512 + (e % 32 / 8 * 16 + col) * 8 + e % 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = top < INFINITY ? v[ks][i] * inv : 0.0f;
+        for (int r = 0; r < 4; ++r) {
+            const float x = finite ? v[i + r] * inv : 0.0f;
             const _Float16 hi = (_Float16)x;
-            out.hi[ks][i] = hi;
-            out.lo[ks][i] = (_Float16)(x - (float)hi);
+            out.pairs[0][at + r] = hi;
+            out.pairs[1][at + r] = (_Float16)(x - (float)hi);
         }
+    }
 }
 
-// One full block of int8 codes. Both products run in integers: the query and
-// the probabilities are three int8 digits each, so their products with the
-// codes are exact, and what is rounded is one fixed-point step of 24 bits.
-template <int HDP, bool MASK>
-__device__ __forceinline__ void codes_block(const uint8_t* block, float2 sc, const Digits<HDP>& qd, int seen,
-                                            Running<HDP>& run) {
-    constexpr int KS = HDP / 64, NT = HDP / 16;
-    const int lane = threadIdx.x % WAVE;
-    const uint8_t* at = block + lane * 16;
-    v4i kf[4 * KS], vf[NT];
-#pragma unroll
-    for (int i = 0; i < 4 * KS; ++i) kf[i] = *(const TRIT_GLOBAL v4i*)(at + i * 1024);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) vf[i] = *(const TRIT_GLOBAL v4i*)(at + BLOCK_TOKENS * HDP + i * 1024);
-    float u[16];
+// Values that are computed here. (The compiler otherwise moves the end of a
+// product behind the branch around the next block's loads, where its integer
+// parts and those loads' registers together spill, and a reload in the loop
+// waits for every load.)
+__device__ __forceinline__ void pin(v4f& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void pin(float& a, float& b, float& c, float& d) {
+    asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+
+__device__ __forceinline__ v4i load16(const uint8_t* p) { return *(const TRIT_GLOBAL v4i*)p; }
+
+// A full block of int8 codes, its keys' and values' fragments in registers.
+// Both products run in integers: the query and the probabilities are three
+// int8 digits each, so their products with the codes are exact, and what is
+// rounded is one fixed-point step of 24 bits.
+template <int HDP>
+__device__ __forceinline__ void codes_scores(const v4i (&kf)[HDP / 16], const v4i (&qd)[3][HDP / 64], float (&u)[16]) {
+    constexpr int KS = HDP / 64;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         v4i c[3];
@@ -214,33 +218,33 @@ __device__ __forceinline__ void codes_block(const uint8_t* block, float2 sc, con
             c[j] = v4i{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                c[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t * KS + ks], qd.d[j][ks], c[j], 0, 0, 0);
+                c[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t * KS + ks], qd[j][ks], c[j], 0, 0, 0);
         }
         // |c| <= 128 * 127 * 128: c1 * 256 + c0 stays within 32 bits.
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             u[4 * t + r] = __builtin_fmaf((float)c[2][r], 65536.0f, (float)((c[1][r] << 8) + c[0][r]));
+        pin(u[4 * t], u[4 * t + 1], u[4 * t + 2], u[4 * t + 3]);
     }
-    float before, now;
-    const bool any = block_softmax<MASK>(u, qd.step * sc.x, seen, run.m, run.l, before, now);
+}
+template <int HDP>
+__device__ __forceinline__ void codes_values(const v4i (&vf)[HDP / 16], const float (&p)[16], float w,
+                                             Running<HDP>& run) {
     v4i pd[3];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         uint32_t x[4];
         // round(p * FIXED) in the low bits of a float of exponent 2^23.
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            x[r] = __builtin_bit_cast(uint32_t, __builtin_fmaf(u[4 * t + r], FIXED, 8388608.0f));
+        for (int r = 0; r < 4; ++r) x[r] = __float_as_uint(__builtin_fmaf(p[4 * t + r], FIXED, 8388608.0f));
         int d0, d1, d2;
         digits4(x[0], x[1], x[2], x[3], d0, d1, d2);
         pd[0][t] = d0;
         pd[1][t] = d1;
         pd[2][t] = d2;
     }
-    // A column that sees nothing of the block takes nothing of it, also where its scale is NaN.
-    const float w = any ? now * sc.y * (1.0f / FIXED) : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < HDP / 16; ++n) {
         v4i c[3];
 #pragma unroll
         for (int j = 0; j < 3; ++j)
@@ -248,8 +252,9 @@ __device__ __forceinline__ void codes_block(const uint8_t* block, float2 sc, con
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float o = __builtin_fmaf((float)c[2][r], 65536.0f, (float)((c[1][r] << 8) + c[0][r]));
-            run.acc[n][r] = __builtin_fmaf(o, w, run.acc[n][r] * before);
+            run.acc[n][r] = __builtin_fmaf(o, w, run.acc[n][r]);
         }
+        pin(run.acc[n]);
     }
 }
 
@@ -261,94 +266,111 @@ __device__ __forceinline__ bool any_nan(v8h x) {
     return hit != 0;
 }
 
-// One f16 block of `tokens` valid ones. CHECK: its values behind the last
-// token are left from other sequences, and a NaN among the valid ones counts
-// for the columns that see its token and no others.
-template <int HDP, bool CHECK>
-__device__ __forceinline__ void f16_block(const _Float16* block, int tokens, const Pairs<HDP>& qp, int seen,
-                                          Running<HDP>& run) {
-    constexpr int KS = HDP / 32, NT = HDP / 16;
-    const int lane = threadIdx.x % WAVE, lq = lane / 16;
-    const _Float16* at = block + lane * 8;
-    v8h kf[4 * KS], vf[NT * 2];
+__device__ __forceinline__ v8h load8h(const _Float16* p) { return *(const TRIT_GLOBAL v8h*)p; }
+
+// An f16 block, the queries (from shared memory) and probabilities as f16 pairs.
+template <int HDP>
+__device__ __forceinline__ void f16_scores(const v8h (&kf)[HDP / 8], const _Float16* hi, const _Float16* lo,
+                                           float (&u)[16]) {
+    constexpr int KS = HDP / 32;
+    const int lane = threadIdx.x % WAVE;
+    v4f c[4];
 #pragma unroll
-    for (int i = 0; i < 4 * KS; ++i) kf[i] = *(const TRIT_GLOBAL v8h*)(at + i * 512);
+    for (int t = 0; t < 4; ++t) c[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < NT * 2; ++i) vf[i] = *(const TRIT_GLOBAL v8h*)(at + BLOCK_TOKENS * HDP + i * 512);
-    float u[16];
+    for (int ks = 0; ks < KS; ++ks) {
+        const v8h qh = *(const v8h*)(hi + ks * 512 + lane * 8), ql = *(const v8h*)(lo + ks * 512 + lane * 8);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            c[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t * KS + ks], ql, c[t], 0, 0, 0);
+            c[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t * KS + ks], qh, c[t], 0, 0, 0);
+        }
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        pin(c[t]);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t * KS + ks], qp.lo[ks], c, 0, 0, 0);
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t * KS + ks], qp.hi[ks], c, 0, 0, 0);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) u[4 * t + r] = c[r];
+        for (int r = 0; r < 4; ++r) u[4 * t + r] = c[t][r];
     }
-    float before, now;
-    const int limit = seen < tokens ? seen : tokens;
-    block_softmax<true>(u, qp.step, limit, run.m, run.l, before, now);
-    v8h ph[2], pl[2];
+}
+__device__ __forceinline__ void value_pairs(const float (&p)[16], v8h (&ph)[2], v8h (&pl)[2]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float p = u[i] * PAIR;
-        const _Float16 hi = (_Float16)p;
+        const float x = p[i] * PAIR;
+        const _Float16 hi = (_Float16)x;
         ph[i / 8][i % 8] = hi;
-        pl[i / 8][i % 8] = (_Float16)(p - (float)hi);
+        pl[i / 8][i % 8] = (_Float16)(x - (float)hi);
     }
+}
+template <int HDP>
+__device__ __forceinline__ void f16_values(const v8h (&vf)[HDP / 8], const float (&p)[16], float now,
+                                           Running<HDP>& run) {
+    v8h ph[2], pl[2];
+    value_pairs(p, ph, pl);
     const float w = now * (1.0f / PAIR);
-    bool nans = false;
-    if (CHECK) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool valid = 32 * s + 16 * (i / 4) + 4 * lq + i % 4 < tokens;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    if (!valid) vf[2 * n + s][i] = (_Float16)0.0f;
-            }
-#pragma unroll
-        for (int i = 0; i < 2 * NT; ++i) nans |= any_nan(vf[i]);
-        nans = __ballot(nans) != 0;
-    }
-    // Which of the lane's tokens its column sees, as f16 ones.
-    v8h sees[2];
-    if (CHECK && nans) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            sees[i / 8][i % 8] = (_Float16)(16 * (i / 4) + 4 * lq + i % 4 < limit ? 1.0f : 0.0f);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < HDP / 16; ++n) {
         v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        if (CHECK && nans) {
-            v4f count = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                v8h is;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool nan = vf[2 * n + s][i] != vf[2 * n + s][i];
-                    is[i] = (_Float16)(nan ? 1.0f : 0.0f);
-                    if (nan) vf[2 * n + s][i] = (_Float16)0.0f;
-                }
-                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees[s], count, 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (count[r] > 0.0f) c[r] = NAN;
-        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[2 * n + s], pl[s], c, 0, 0, 0);
             c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[2 * n + s], ph[s], c, 0, 0, 0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) run.acc[n][r] = __builtin_fmaf(c[r], w, run.acc[n][r] * before);
+        for (int r = 0; r < 4; ++r) run.acc[n][r] = __builtin_fmaf(c[r], w, run.acc[n][r]);
+        pin(run.acc[n]);
     }
+}
+
+// A sequence's open block: values behind its last token are left from other
+// sequences and taken as 0; a NaN among the valid ones counts for the columns
+// that see its token and no others -- found by a product of its own.
+template <int HDP>
+__device__ __forceinline__ void open_values(v8h (&vf)[HDP / 8], const float (&p)[16], float now, int tokens, int seen,
+                                            Running<HDP>& run) {
+    constexpr int NT = HDP / 16;
+    const int lq = (threadIdx.x % WAVE) / 16;
+    bool nans = false;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        // The lane's tokens of this half that are valid, as a mask of its 8 halves.
+        v4i keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = 32 * s + 16 * (i / 2) + 4 * lq + 2 * (i % 2);
+            keep[i] = t + 1 < tokens ? -1 : t < tokens ? 0xffff : 0;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            vf[2 * n + s] = __builtin_bit_cast(v8h, __builtin_bit_cast(v4i, vf[2 * n + s]) & keep);
+            nans |= any_nan(vf[2 * n + s]);
+        }
+    }
+    if (__any(nans)) {
+        v8h sees[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sees[i / 8][i % 8] = (_Float16)(16 * (i / 4) + 4 * lq + i % 4 < min(seen, tokens) ? 1.0f : 0.0f);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            v4f count = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                v8h is;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const _Float16 x = vf[2 * n + s][i];
+                    is[i] = (_Float16)(x != x ? 1.0f : 0.0f);
+                    vf[2 * n + s][i] = x != x ? (_Float16)0.0f : x;
+                }
+                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees[s], count, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.0f) run.acc[n][r] = NAN;
+        }
+    }
+    f16_values<HDP>(vf, p, now, run);
 }
 
 __global__ void clear_kernel(int* p, int n) {
@@ -374,74 +396,155 @@ __device__ __forceinline__ float2 get(const float* p) {
 // memory. Of the workgroups of a tile's chunks the last to end joins theirs,
 // in the chunks' order.
 template <int HDP, bool PAGED>
-__global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
-    constexpr int NT = HDP / 16;
+__global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
+    constexpr int NT = HDP / 16, KS = HDP / 64, PS = HDP + 4;
+    constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
+    __shared__ Queries<HDP, PAGED> qs;
     __shared__ float top[WAVES][16], sum[WAVES][16];
-    __shared__ float part[WAVES][16][HDP];
+    __shared__ __align__(16) float part[WAVES][16][PS];
     __shared__ bool arrived;
-    const int t = threadIdx.x, w = t / WAVE, lane = t % WAVE, col = lane % 16, lq = lane / 16;
-    // The last sequence whose items start at or before this one.
+    const int t = threadIdx.x, lane = t % WAVE, col = lane % 16, lq = lane / 16;
+    const int w = __builtin_amdgcn_readfirstlane(t / WAVE);
+    // The last sequence whose items start at or before this one (the starts behind the last are past every item).
+    const int g = blockIdx.x;
     int si = 0;
 #pragma unroll
-    for (int i = 0; i < CALL_SEQS; i += WAVE)
-        si += __popcll(__ballot(i + lane < a.n && a.s[i + lane].start <= (int)blockIdx.x));
+    for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
     const AttendSeq seq = a.s[si - 1];
-    const int item = (int)blockIdx.x - seq.start;
-    const int g = item % a.kv_heads, chunk = item / a.kv_heads % seq.chunks, tile = item / a.kv_heads / seq.chunks;
-    const int columns = seq.rows * a.group;
-    const int c = tile * 16 + col, row = c / a.group;
-    const int head = g * a.group + c % a.group;
-    const float* q = c < columns ? a.q + (size_t)(seq.first + row) * a.qs + (size_t)head * a.hd : nullptr;
-    // Keys the column sees; the tile's most and least.
-    const int ahead = PAGED ? seq.len - seq.rows + 1 : seq.len;
-    const int last = (tile * 16 + 15 < columns ? tile * 16 + 15 : columns - 1) / a.group;
-    const int most = PAGED ? ahead + last : ahead, least = PAGED ? ahead + tile * 16 / a.group : ahead;
-    const int seen = c < columns ? (PAGED ? ahead + row : ahead) : 0;
+    const int item = (int)blockIdx.y - seq.start;
+    const int tile = seq.chunks == 1 ? item : item / seq.chunks, chunk = item - tile * seq.chunks;
+    const int columns = seq.rows * a.group, cols = min(columns - tile * 16, 16);
+    // Column c's row and head: row0 + (rest + c) / group. The quotient is of small whole numbers, exact in f32.
+    const int row0 = tile * 16 / a.group, rest = tile * 16 - row0 * a.group;
+    const float per = 1.0f / (float)a.group;
+    auto row_of = [&](int c) { return (int)(((float)(rest + c) + 0.5f) * per); };
+
+    // The thread's query values are on their way while the first keys are.
+    float qv[NT];
+    {
+        const int c = t / 16, r = row_of(c), h = g * a.group + rest + c - r * a.group;
+        const bool valid = c < cols;
+        load_queries<HDP, PAGED>(valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q, valid,
+                                 a.aligned, a.hd, a.scale, qv);
+    }
+    // Keys the lane's column sees, and the tile's most and least.
+    const int ahead = PAGED ? seq.len - seq.rows + 1 + row0 : seq.len;
+    const int most = PAGED ? ahead + (rest + cols - 1) / a.group : ahead;
+    const int seen = PAGED ? ahead + row_of(min(col, cols - 1)) : ahead;
     const int b0 = chunk * a.chunk;
     const int all = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS, end = all < b0 + a.chunk ? all : b0 + a.chunk;
 
     Running<HDP> run;
     run.clear();
+    int b = b0 + w;
     if constexpr (PAGED) {
         const int full = seq.len / BLOCK_TOKENS;  // full blocks hold codes
+        const int last = end < full ? end : full;
         const int* table = a.table + (size_t)seq.place * a.table_stride;
-        Digits<HDP> qd;
-        query_digits<HDP>(q, a.hd, a.scale, qd);
-        int b = b0 + w;
-        for (; b < end && b < full; b += WAVES) {
-            const size_t at = (size_t)table[b] * a.kv_heads + g;
-            const uint8_t* block = a.codes + at * (2 * BLOCK_TOKENS * HDP);
-            const float2 sc = a.scales[at];
-            if ((b + 1) * BLOCK_TOKENS <= least)
-                codes_block<HDP, false>(block, sc, qd, 0, run);
-            else
-                codes_block<HDP, true>(block, sc, qd, seen - b * BLOCK_TOKENS, run);
+        v4i kf[NT], vf[NT];
+        float2 sc = make_float2(0.0f, 0.0f);
+        int page = b < last ? table[b] : 0;
+        const uint8_t* block = nullptr;
+        if (b < last) {
+            const size_t at = (size_t)page * a.kv_heads + g;
+            block = a.codes + at * BLOCK + lane * 16;
+            sc = a.scales[at];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) kf[i] = load16(block + i * 1024);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024);
+            page = b + WAVES < last ? table[b + WAVES] : 0;
+        }
+        put_queries<HDP, PAGED>(qv, qs);
+        __syncthreads();
+        v4i qd[3][KS];
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qd[j][ks] = *(const v4i*)(qs.digits[j] + ks * 1024 + lane * 16);
+        const float step = qs.top[col] * (LOG2E / FIXED);
+        for (; b < last; b += WAVES) {
+            float u[16];
+            codes_scores<HDP>(kf, qd, u);
+            const bool more = b + WAVES < last;
+            const float2 s0 = sc;
+            const uint8_t* next = block;
+            if (more) {
+                const size_t at = (size_t)page * a.kv_heads + g;
+                next = a.codes + at * BLOCK + lane * 16;
+                sc = a.scales[at];
+                page = b + 2 * WAVES < last ? table[b + 2 * WAVES] : 0;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024);
+            }
+            const float now =
+                block_softmax<HDP>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > ahead, seen - b * BLOCK_TOKENS, run);
+            // A column that sees nothing of the block takes nothing of it, also where its scale is NaN.
+            codes_values<HDP>(vf, u, now == 0.0f && seen <= b * BLOCK_TOKENS ? 0.0f : now * s0.y * (1.0f / FIXED), run);
+            if (more) {
+                block = next;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024);
+            }
         }
         if (b < end) {
-            Pairs<HDP> qp;
-            query_pairs<HDP>(q, a.hd, a.scale, qp);
-            const _Float16* block = a.f16 + ((size_t)seq.place * a.kv_heads + g) * (2 * BLOCK_TOKENS * HDP);
-            f16_block<HDP, true>(block, seq.len - b * BLOCK_TOKENS, qp, seen - b * BLOCK_TOKENS, run);
+            const _Float16* open = a.f16 + ((size_t)seq.place * a.kv_heads + g) * BLOCK + lane * 8;
+            v8h k16[2 * NT], v16[2 * NT];
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) k16[i] = load8h(open + i * 512);
+            float u[16];
+            const int tokens = seq.len - b * BLOCK_TOKENS, sees = seen - b * BLOCK_TOKENS;
+            f16_scores<HDP>(k16, qs.pairs[0], qs.pairs[1], u);
+            // (With the values' loads before the scores' products the 128-wide kernel spills.)
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) v16[i] = load8h(open + BLOCK / 2 + i * 512);
+            const float now = block_softmax<HDP>(u, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
+            open_values<HDP>(v16, u, now, tokens, sees, run);
         }
     } else {
-        Pairs<HDP> qp;
-        query_pairs<HDP>(q, a.hd, a.scale, qp);
-        const _Float16* states = a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * (2 * BLOCK_TOKENS * HDP);
-        for (int b = b0 + w; b < end; b += WAVES)
-            f16_block<HDP, false>(states + (size_t)b * (2 * BLOCK_TOKENS * HDP), seq.len - b * BLOCK_TOKENS, qp,
-                                  seq.len - b * BLOCK_TOKENS, run);
+        const _Float16* states =
+            a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * BLOCK + lane * 8;
+        // 64 wide, the next block's values are on their way too; 128 wide they would not fit the registers.
+        constexpr bool AHEAD = HDP == 64;
+        v8h kf[2 * NT], vf[2 * NT];
+        auto load = [&](v8h(&f)[2 * NT], int at, int half) {
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) f[i] = load8h(states + at * BLOCK + half * (BLOCK / 2) + i * 512);
+        };
+        if (b < end) {
+            load(kf, b, 0);
+            if (AHEAD) load(vf, b, 1);
+        }
+        put_queries<HDP, PAGED>(qv, qs);
+        __syncthreads();
+        const float step = qs.top[col] * (LOG2E / PAIR);
+        for (; b < end; b += WAVES) {
+            float u[16];
+            f16_scores<HDP>(kf, qs.pairs[0], qs.pairs[1], u);
+            if (!AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);
+                load(vf, b, 1);
+            }
+            const bool more = b + WAVES < end;
+            if (more && AHEAD) load(kf, b + WAVES, 0);
+            const float now =
+                block_softmax<HDP>(u, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
+            f16_values<HDP>(vf, u, now, run);
+            if (more && !AHEAD) load(kf, b + WAVES, 0);
+            if (more && AHEAD) load(vf, b + WAVES, 1);
+        }
     }
     const float lsum = column_sum(run.l);
     if (lq == 0) {
         top[w][col] = run.m;
         sum[w][col] = lsum;
     }
+    if (col < cols) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) part[w][col][16 * n + 4 * lq + r] = run.acc[n][r];
+        for (int n = 0; n < NT; ++n) *(v4f*)(part[w][col] + 16 * n + 4 * lq) = run.acc[n];
+    }
     __syncthreads();
-    const int cols = min(columns - tile * 16, 16);
     // The sums of the waves' parts, relative to their largest score m.
     auto joined = [&](int cc, int e, float& m, float& l) {
         m = top[0][cc];
@@ -459,9 +562,10 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
         return o;
     };
     auto store = [&](int cc, int e, float o, float l) {
-        const int rr = (tile * 16 + cc) / a.group, hh = g * a.group + (tile * 16 + cc) % a.group;
+        const int r = row_of(cc), h = g * a.group + rest + cc - r * a.group;
         // No key at all: 0.
-        if (e < a.hd) a.out[((size_t)(seq.first + rr) * a.kv_heads * a.group + hh) * a.hd + e] = l == 0.0f ? 0.0f : o / l;
+        if (e < a.hd)
+            a.out[((size_t)(seq.first + row0 + r) * a.kv_heads * a.group + h) * a.hd + e] = l == 0.0f ? 0.0f : o / l;
     };
     if (seq.chunks == 1) {
         for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
@@ -475,14 +579,14 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
         const int cc = i / HDP, e = i % HDP;
         float m, l;
         const float o = joined(cc, e, m, l);
-        const size_t at = (size_t)blockIdx.x * 16 + cc;
+        const size_t at = ((size_t)blockIdx.y * a.kv_heads + g) * 16 + cc;
         put(a.sums + at * HDP + e, o);
         if (e == 0) put(a.tops + at, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(m));
     }
     // Every store of the workgroup is in memory before its arrival is counted.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    int* counter = a.counters + seq.group + tile * a.kv_heads + g;
+    int* counter = a.counters + (seq.group + tile) * a.kv_heads + g;
     if (t == 0) {
         const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         arrived = before + 1 == seq.chunks;
@@ -491,7 +595,7 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
     __syncthreads();
     if (!arrived) return;
     // Chunk v's item; wave w joins the chunks w, w + 4, .. of each column, lane l their elements 2 l, 2 l + 1.
-    const size_t first = (size_t)seq.start + (size_t)tile * seq.chunks * a.kv_heads + g;
+    const size_t first = (size_t)(seq.start + tile * seq.chunks) * a.kv_heads + g;
     for (int cc = 0; cc < cols; ++cc) {
         float m = -INFINITY, l = 0.0f;
         float2 o = make_float2(0.0f, 0.0f);
@@ -527,9 +631,9 @@ __global__ __launch_bounds__(WAVES * WAVE) void attend_kernel(AttendArgs a) {
 
 }  // namespace
 
-// Items of one launch (a grid holds fewer than 2^32 threads), and the most
-// where keys are split: what the scratch holds.
-constexpr long long MOST_ITEMS = 1 << 23;
+// Tiles of one launch (65535 blocks in the grid's second dimension), and the
+// most workgroups where keys are split: what the scratch holds.
+constexpr long long MOST_TILES = 65535;
 constexpr long long SPLIT_ITEMS = 1024;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
@@ -547,41 +651,41 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     a.counters = (int*)(a.tops + SPLIT_ITEMS * 16);
     const auto tiles = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 15) / 16; };
     const auto blocks = [](const AttendSeq& q) { return (q.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS; };
+    a.aligned = a.hd % 4 == 0 && a.qs % 4 == 0 && (uintptr_t)a.q % 16 == 0;
     for (size_t from = 0; from < seqs.size();) {
         // The launch's sequences, and its work in blocks of keys.
         long long whole = 0, work = 0;
         size_t to = from;
         for (a.n = 0; to < seqs.size() && a.n < CALL_SEQS; ++to) {
             if (seqs[to].rows == 0) continue;
-            const long long items = tiles(seqs[to]) * a.kv_heads;
-            if (items > MOST_ITEMS) fail("attention: more query rows than one launch takes");
-            if (a.n && whole + items > MOST_ITEMS) break;
-            whole += items;
-            work += items * blocks(seqs[to]);
+            if (tiles(seqs[to]) > MOST_TILES) fail("attention: more query rows than one launch takes");
+            if (a.n && whole + tiles(seqs[to]) > MOST_TILES) break;
+            whole += tiles(seqs[to]);
+            work += tiles(seqs[to]) * blocks(seqs[to]);
             a.s[a.n++] = seqs[to];
         }
         from = to;
         if (!a.n) return;
         // Chunks of as few blocks as keep the items within the scratch, a multiple of what the waves take at once.
-        long long items = whole;
         a.chunk = INT_MAX / 2;
-        if (whole < SPLIT_ITEMS) {
-            const long long room = SPLIT_ITEMS - whole;
-            a.chunk = (int)((work + room - 1) / room + WAVES - 1) / WAVES * WAVES;
-            if (a.chunk < WAVES) a.chunk = WAVES;
-        }
-        items = 0;
-        int groups = 0;
-        for (int i = 0; i < a.n; ++i) {
+        const long long room = SPLIT_ITEMS / a.kv_heads - whole;
+        if (room > 0) a.chunk = (int)((work + room - 1) / room + WAVES - 1) / WAVES * WAVES;
+        if (a.chunk < WAVES) a.chunk = WAVES;
+        int items = 0, groups = 0;
+        for (int i = 0; i < CALL_SEQS; ++i) {
             AttendSeq& q = a.s[i];
+            if (i >= a.n) {
+                q.start = INT_MAX;
+                continue;
+            }
             const int nb = blocks(q);
             q.chunks = nb <= a.chunk ? 1 : (nb + a.chunk - 1) / a.chunk;
-            q.start = (int)items;
+            q.start = items;
             q.group = groups;
-            items += tiles(q) * a.kv_heads * q.chunks;
-            if (q.chunks > 1) groups += (int)tiles(q) * a.kv_heads;
+            items += (int)tiles(q) * q.chunks;
+            if (q.chunks > 1) groups += (int)tiles(q);
         }
-        const dim3 grid((unsigned)items), block(WAVES * WAVE);
+        const dim3 grid((unsigned)a.kv_heads, (unsigned)items), block(WAVES * WAVE);
         if (hdp == 64) {
             if (paged)
                 hipLaunchKernelGGL((attend_kernel<64, true>), grid, block, 0, s, a);
