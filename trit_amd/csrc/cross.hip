@@ -6,13 +6,14 @@
 
 #include "../../include/trit_hip.h"
 #include "attend.h"
+#include "blocks.h"
 #include "device.h"
 #include "internal.h"
 
 namespace trit {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = BLOCK_THREADS;
 
 struct SetSeq {
     int slot, keys;
@@ -27,23 +28,35 @@ struct SetArgs {
 // keys that are not there meet probabilities of 0.)
 template <int HDP>
 __global__ __launch_bounds__(THREADS) void set_kernel(_Float16* states, int blocks, int kv_heads, int hd, SetArgs a,
-                                                      const float* k, long long ks, const float* v, long long vs) {
+                                                      const float* k, long long ks, const float* v, long long vs,
+                                                      bool aligned) {
+    constexpr int G = BlockShare<HDP>::GROUPS;
     __shared__ __align__(16) _Float16 out[BLOCK_TOKENS * HDP];
-    const int which = blockIdx.z % 2, g = blockIdx.y, t = threadIdx.x, x = blockIdx.x;
+    const bool which = blockIdx.z % 2;
+    const int g = blockIdx.y, t = threadIdx.x, first = blockIdx.x * BLOCK_TOKENS;
     const SetSeq s = a.s[blockIdx.z / 2];
-    if (x * BLOCK_TOKENS >= s.keys) return;
-    const float* rows = which ? v : k;
+    if (first >= s.keys) return;
     const long long stride = which ? vs : ks;
-    for (int i = t; i < BLOCK_TOKENS * HDP; i += THREADS) {
-        const int tok = i / HDP, e = i % HDP, key = x * BLOCK_TOKENS + tok;
-        float y = 0.0f;
-        if (key < s.keys && e < hd) y = rows[(size_t)(s.first + key) * stride + (size_t)g * hd + e];
-        const _Float16 h = (_Float16)y;
-        out[which ? v16_at<HDP>(tok, e) : k16_at<HDP>(tok, e)] = __builtin_fabsf((float)h) < INFINITY ? h : (_Float16)NAN;
+    float h[4 * G];
+    load_share<HDP>(which, (which ? v : k) + (size_t)s.first * stride + (size_t)g * hd, stride, first, s.keys, hd,
+                    aligned, h);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        int tok, e;
+        share_at<HDP>(which, i, tok, e);
+        _Float16 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool valid = first + tok + (which ? j : 0) < s.keys && e + (which ? 0 : j) < hd;
+            x[j] = valid ? held(h[4 * i + j]) : (_Float16)0.0f;
+        }
+        __builtin_memcpy(out + half_at<HDP>(which, tok, e), x, 8);
     }
     __syncthreads();
-    uint4* dst = (uint4*)(states + ((((size_t)s.slot * kv_heads + g) * blocks + x) * 2 + which) * (BLOCK_TOKENS * HDP));
-    for (int i = t; i < BLOCK_TOKENS * HDP / 8; i += THREADS) dst[i] = *(const uint4*)(out + i * 8);
+    uint4* dst =
+        (uint4*)(states + ((((size_t)s.slot * kv_heads + g) * blocks + blockIdx.x) * 2 + which) * (BLOCK_TOKENS * HDP));
+#pragma unroll
+    for (int i = 0; i < BLOCK_TOKENS * HDP / 8; i += THREADS) dst[i + t] = *(const uint4*)(out + (i + t) * 8);
 }
 
 }  // namespace
@@ -182,7 +195,9 @@ int trit_hip_cross_set_device(TritHipCross* cross, int layer, const int32_t* slo
             auto kernel = cross->hdp == 64 ? set_kernel<64> : set_kernel<128>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)most, (unsigned)cross->kv_heads, (unsigned)(2 * m)), dim3(THREADS),
                                0, s, cross->states.as<_Float16>() + (size_t)layer * cross->layer_values(), cross->blocks,
-                               cross->kv_heads, cross->hd, a, k, (long long)k_stride, v, (long long)v_stride);
+                               cross->kv_heads, cross->hd, a, k, (long long)k_stride, v, (long long)v_stride,
+                               cross->hd % 4 == 0 && k_stride % 4 == 0 && v_stride % 4 == 0 &&
+                                   ((uintptr_t)k | (uintptr_t)v) % 16 == 0);
             TRIT_HIP(hipGetLastError());
         }
         return 0;

@@ -7,6 +7,7 @@
 
 #include "../../include/trit_hip.h"
 #include "attend.h"
+#include "blocks.h"
 #include "device.h"
 #include "internal.h"
 #include "page_book.h"
@@ -16,7 +17,7 @@ namespace {
 
 static_assert(PageBook::BLOCK == BLOCK_TOKENS, "one block size");
 
-constexpr int THREADS = 256;
+constexpr int THREADS = BLOCK_THREADS;
 // Entries of one launch (kernel arguments).
 constexpr int CALL_ENTRIES = 256;
 
@@ -45,12 +46,6 @@ struct RowsArgs {
     RowsSeq s[CALL_SEQS];
 };
 
-// f16 as the cache holds it: what f16 does not hold as a finite value is NaN.
-__device__ __forceinline__ _Float16 held(float v) {
-    const _Float16 h = (_Float16)v;
-    return __builtin_fabsf((float)h) < INFINITY ? h : (_Float16)NAN;
-}
-
 // round(127 h / a), halves to even. 127 h is exact; the product with the
 // reciprocal is off by less than 1e-4, so only quotients that near a half are
 // divided, and no quotient of two f16 values rounds onto a half it is not.
@@ -68,79 +63,97 @@ __device__ __forceinline__ int block_code(float h, float a, float inv) {
 // alone reads the open block's old rows, which the last block replaces.
 template <int HDP>
 __global__ __launch_bounds__(THREADS) void append_kernel(Pool p, RowsArgs a, const float* k, long long ks,
-                                                         const float* v, long long vs) {
-    constexpr int EACH = BLOCK_TOKENS * HDP / THREADS;  // values a thread
+                                                         const float* v, long long vs, bool aligned) {
+    constexpr int G = BlockShare<HDP>::GROUPS, VALUES = BlockShare<HDP>::VALUES;
     __shared__ __align__(16) uint32_t codes[BLOCK_TOKENS * HDP / 4];
     __shared__ float red[THREADS / WAVE];
-    __shared__ int nan_seen;
-    const int which = blockIdx.z % 2, g = blockIdx.y, t = threadIdx.x;
+    __shared__ bool nan_seen[THREADS / WAVE];
+    const int g = blockIdx.y, t = threadIdx.x, x = blockIdx.x;
+    const bool which = blockIdx.z % 2;
     const RowsSeq s = a.s[blockIdx.z / 2];
     const int b0 = s.len / BLOCK_TOKENS, have = s.len % BLOCK_TOKENS;
     const int touched = (have + s.count + BLOCK_TOKENS - 1) / BLOCK_TOKENS;  // blocks
-    if (s.count == 0 || (int)blockIdx.x >= touched) return;
+    if (s.count == 0 || x >= touched) return;
     const bool ends_full = (have + s.count) % BLOCK_TOKENS == 0;
-    const float* rows = which ? v : k;
     const long long stride = which ? vs : ks;
+    const float* rows = (which ? v : k) + (size_t)s.first * stride + (size_t)g * p.hd;
     _Float16* open = p.open + (((size_t)s.row * p.kv_heads + g) * 2 + which) * (BLOCK_TOKENS * HDP);
-    // The value at token `tok` of block b0 + x, as held.
-    auto value = [&](int x, int tok, int e) -> _Float16 {
-        if (e >= p.hd) return (_Float16)0.0f;
-        const int i = x * BLOCK_TOKENS + tok - have;  // of the call's rows
-        if (i < 0) return open[which ? v16_at<HDP>(tok, e) : k16_at<HDP>(tok, e)];
-        return held(rows[(size_t)(s.first + i) * stride + (size_t)g * p.hd + e]);
-    };
-    const int x = blockIdx.x;
     if (x + 1 < touched || ends_full) {
-        // A thread's values lie side by side in the code order: 4 dims of a
-        // token (keys), or 4 tokens of a dim (values).
-        float h[EACH];
+        float h[VALUES];
+        load_share<HDP>(which, rows, stride, x * BLOCK_TOKENS - have, s.count, p.hd, aligned, h);
+        if (x == 0 && have) {
+            // The tokens that the open block holds.
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                int tok, e;
+                share_at<HDP>(which, i, tok, e);
+                _Float16 old[4];
+                const uint2 o = gload_u2(open + half_at<HDP>(which, tok, e));
+                __builtin_memcpy(old, &o, 8);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (tok + (which ? j : 0) < have) h[4 * i + j] = (float)old[j];
+            }
+        }
         float top = 0.0f;
         bool nan = false;
 #pragma unroll
-        for (int i = 0; i < EACH; i += 4) {
-            const int u = t + i / 4 * THREADS;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int tok = which ? u / HDP * 4 + j : u / (HDP / 4);
-                const int e = which ? u % HDP : u % (HDP / 4) * 4 + j;
-                h[i + j] = (float)value(x, tok, e);
-                top = __builtin_fmaxf(top, __builtin_fabsf(h[i + j]));
-                nan |= h[i + j] != h[i + j];
-            }
+        for (int i = 0; i < VALUES; ++i) {
+            int tok, e;
+            share_at<HDP>(which, i / 4, tok, e);
+            h[i] = (which ? e : e + i % 4) < p.hd ? (float)held(h[i]) : 0.0f;
+            top = __builtin_fmaxf(top, __builtin_fabsf(h[i]));
+            nan |= h[i] != h[i];
         }
-        if (t == 0) nan_seen = 0;
 #pragma unroll
         for (int m = 1; m < WAVE; m <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, m));
-        if (t % WAVE == 0) red[t / WAVE] = top;
-        __syncthreads();
-        if (nan) nan_seen = 1;
+        nan = __any(nan);
+        if (t % WAVE == 0) {
+            red[t / WAVE] = top;
+            nan_seen[t / WAVE] = nan;
+        }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < THREADS / WAVE; ++w) top = __builtin_fmaxf(top, red[w]);
-        const bool bad = nan_seen != 0;
+        for (int w = 0; w < THREADS / WAVE; ++w) {
+            top = __builtin_fmaxf(top, red[w]);
+            nan |= nan_seen[w];
+        }
         const float inv = 1.0f / top;
 #pragma unroll
-        for (int i = 0; i < EACH; i += 4) {
-            const int u = t + i / 4 * THREADS;
-            int c[4];
+        for (int i = 0; i < G; ++i) {
+            int tok, e, c[4];
+            share_at<HDP>(which, i, tok, e);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] = bad || top == 0.0f ? 0 : block_code(h[i + j], top, inv);
-            const int at = which ? v8_at<HDP>(u / HDP * 4, u % HDP) : k8_at<HDP>(u / (HDP / 4), u % (HDP / 4) * 4);
-            codes[at / 4] = pack4(c[0], c[1], c[2], c[3]);
+            for (int j = 0; j < 4; ++j) c[j] = nan || top == 0.0f ? 0 : block_code(h[4 * i + j], top, inv);
+            codes[code_at<HDP>(which, tok, e) / 4] = pack4(c[0], c[1], c[2], c[3]);
         }
         __syncthreads();
         const size_t page = (size_t)p.table[(size_t)s.row * p.pages + b0 + x] * p.kv_heads + g;
         uint4* dst = (uint4*)(p.codes + (page * 2 + which) * (BLOCK_TOKENS * HDP));
-        for (int i = t; i < BLOCK_TOKENS * HDP / 16; i += THREADS) dst[i] = *(const uint4*)(codes + i * 4);
-        if (t == 0) (which ? p.scales[page].y : p.scales[page].x) = bad ? NAN : top / 127.0f;
+#pragma unroll
+        for (int i = 0; i < BLOCK_TOKENS * HDP / 16; i += THREADS) dst[i + t] = *(const uint4*)(codes + (i + t) * 4);
+        if (t == 0) (which ? p.scales[page].y : p.scales[page].x) = nan ? NAN : top / 127.0f;
     }
     // The open block at the end: its own workgroup is the first block's.
     if (x != 0 || ends_full) return;
-    __syncthreads();
-    const int xl = touched - 1, from = xl == 0 ? have : 0, to = (have + s.count) % BLOCK_TOKENS;
-    for (int i = t; i < (to - from) * p.hd; i += THREADS) {
-        const int tok = from + i / p.hd, e = i % p.hd;
-        open[which ? v16_at<HDP>(tok, e) : k16_at<HDP>(tok, e)] = value(xl, tok, e);
+    const int first = (touched - 1) * BLOCK_TOKENS - have, from = max(-first, 0), to = (have + s.count) % BLOCK_TOKENS;
+    if (to - from <= 2) {
+        // A step's one or two rows: a value a thread.
+        const int tok = from + t / HDP, e = t % HDP;
+        if (tok < to && e < p.hd)
+            open[half_at<HDP>(which, tok, e)] = held(rows[(size_t)(first + tok) * stride + e]);
+        return;
+    }
+    float h[VALUES];
+    load_share<HDP>(which, rows, stride, first, s.count, p.hd, aligned, h);
+    __syncthreads();  // the old rows are read
+#pragma unroll
+    for (int i = 0; i < VALUES; ++i) {
+        int tok, e;
+        share_at<HDP>(which, i / 4, tok, e);
+        tok += which ? i % 4 : 0;
+        e += which ? 0 : i % 4;
+        if (tok >= from && tok < to && e < p.hd) open[half_at<HDP>(which, tok, e)] = held(h[i]);
     }
 }
 
@@ -148,8 +161,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(Pool p, RowsArgs a, con
 // x-th block that sequence i's range touches.
 template <int HDP>
 __global__ __launch_bounds__(THREADS) void read_kernel(Pool p, RowsArgs a, float* k, long long ks, float* v,
-                                                       long long vs) {
-    const int which = blockIdx.z % 2, g = blockIdx.y, t = threadIdx.x;
+                                                       long long vs, bool aligned) {
+    const bool which = blockIdx.z % 2;
+    const int g = blockIdx.y, t = threadIdx.x;
     const RowsSeq s = a.s[blockIdx.z / 2];
     const int b = s.at / BLOCK_TOKENS + (int)blockIdx.x;
     const int from = max(s.at - b * BLOCK_TOKENS, 0), to = min(s.at + s.count - b * BLOCK_TOKENS, BLOCK_TOKENS);
@@ -157,23 +171,72 @@ __global__ __launch_bounds__(THREADS) void read_kernel(Pool p, RowsArgs a, float
     float* out = which ? v : k;
     const long long stride = which ? vs : ks;
     const bool full = (b + 1) * BLOCK_TOKENS <= s.len;
-    const _Float16* open = p.open + (((size_t)s.row * p.kv_heads + g) * 2 + which) * (BLOCK_TOKENS * HDP);
-    const int8_t* codes = nullptr;
-    float scale = 0.0f;
+    const int lane = t % WAVE, col = lane % 16, lq = lane / 16;
+    float* rows = out + (s.first + (long long)b * BLOCK_TOKENS - s.at) * stride + (size_t)g * p.hd;
+    auto store = [&](int tok, int e, float x) {
+        if (tok >= from && tok < to && e < p.hd) rows[(size_t)tok * stride + e] = x;
+    };
+    // Four consecutive dims of a token.
+    auto store4 = [&](int tok, int e, float a0, float a1, float a2, float a3) {
+        if (aligned) {
+            if (tok >= from && tok < to && e < p.hd) *(float4*)(rows + (size_t)tok * stride + e) = make_float4(a0, a1, a2, a3);
+        } else {
+            store(tok, e, a0);
+            store(tok, e + 1, a1);
+            store(tok, e + 2, a2);
+            store(tok, e + 3, a3);
+        }
+    };
+    // A wave takes whole 1 KB fragments, 16 bytes a lane, all on their way before the first is used.
     if (full) {
+        constexpr int N = BLOCK_TOKENS * HDP / 16 / THREADS;
         const size_t page = (size_t)p.table[(size_t)s.row * p.pages + b] * p.kv_heads + g;
-        codes = (const int8_t*)p.codes + (page * 2 + which) * (BLOCK_TOKENS * HDP);
-        scale = which ? p.scales[page].y : p.scales[page].x;
+        const uint8_t* codes = p.codes + (page * 2 + which) * (BLOCK_TOKENS * HDP);
+        const float scale = which ? p.scales[page].y : p.scales[page].x;
+        uint4 c[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = gload_u4(codes + (i * THREADS + t) * 16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int f = (i * THREADS + t) / WAVE;
+            const uint32_t words[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = (float)(int8_t)(words[j] >> (8 * r)) * scale;
+                if (which) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) store(16 * j + 4 * lq + r, 16 * f + col, x[r]);
+                } else {
+                    constexpr int KS = HDP / 64;
+                    store4(f / KS * 16 + col, f % KS * 64 + 16 * lq + 4 * j, x[0], x[1], x[2], x[3]);
+                }
+            }
+        }
+        return;
     }
-    for (int i = t; i < (to - from) * HDP; i += THREADS) {
-        const int tok = from + i / HDP, e = i % HDP;
-        if (e >= p.hd) continue;
-        float x;
-        if (full)
-            x = (float)codes[which ? v8_at<HDP>(tok, e) : k8_at<HDP>(tok, e)] * scale;
-        else
-            x = (float)open[which ? v16_at<HDP>(tok, e) : k16_at<HDP>(tok, e)];
-        out[(size_t)(s.first + b * BLOCK_TOKENS + tok - s.at) * stride + (size_t)g * p.hd + e] = x;
+    constexpr int N = BLOCK_TOKENS * HDP / 8 / THREADS;
+    const _Float16* open = p.open + (((size_t)s.row * p.kv_heads + g) * 2 + which) * (BLOCK_TOKENS * HDP);
+    uint4 c[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = gload_u4(open + (i * THREADS + t) * 8);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int f = (i * THREADS + t) / WAVE;
+        _Float16 x[8];
+        __builtin_memcpy(x, &c[i], 16);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (which) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) store(f % 2 * 32 + 16 * j + 4 * lq + r, f / 2 * 16 + col, (float)x[4 * j + r]);
+            } else {
+                constexpr int KS = HDP / 32;
+                store4(f / KS * 16 + col, f % KS * 32 + 8 * lq + 4 * j, (float)x[4 * j], (float)x[4 * j + 1],
+                       (float)x[4 * j + 2], (float)x[4 * j + 3]);
+            }
+        }
     }
 }
 
@@ -199,10 +262,21 @@ __global__ __launch_bounds__(THREADS) void row_kernel(const _Float16* from, int 
             table[(size_t)c.dst * pages + i] = table[(size_t)c.src * pages + i];
     const int tokens = c.len % BLOCK_TOKENS;
     if (!tokens) return;
+    // The 1 KB fragments that hold its tokens: of K whole tiles of 16, of V halves of 32.
     constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
-    const uint4* src = (const uint4*)(from + (((size_t)layer * from_rows + c.src) * kv_heads + g) * BLOCK);
-    uint4* dst = (uint4*)(to + (((size_t)layer * to_rows + c.dst) * kv_heads + g) * BLOCK);
-    for (int i = t; i < (int)(BLOCK / 8); i += THREADS) dst[i] = src[i];
+    constexpr int N = BLOCK / 8 / THREADS, KF = 4 * (HDP / 32);
+    const _Float16* src = from + (((size_t)layer * from_rows + c.src) * kv_heads + g) * BLOCK;
+    _Float16* dst = to + (((size_t)layer * to_rows + c.dst) * kv_heads + g) * BLOCK;
+    auto needed = [&](int i) {
+        const int f = (i * THREADS + t) / WAVE;
+        return f < KF ? f / (HDP / 32) * 16 < tokens : (f - KF) % 2 * 32 < tokens;
+    };
+    uint4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = gload_u4(src + (needed(i) ? (i * THREADS + t) * 8 : t % WAVE * 8));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (needed(i)) *(uint4*)(dst + (i * THREADS + t) * 8) = x[i];
 }
 
 // Pages from one pool to another (or within one: no page is both read and
@@ -218,10 +292,12 @@ __global__ __launch_bounds__(THREADS) void page_kernel(const uint8_t* codes, con
     const int layer = blockIdx.y / kv_heads, g = blockIdx.y % kv_heads, t = threadIdx.x;
     constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
     const size_t src = ((size_t)layer * pages + m.src) * kv_heads + g, dst = ((size_t)layer * to_pages + m.dst) * kv_heads + g;
-    const uint4* from = (const uint4*)(codes + src * BLOCK);
-    uint4* to = (uint4*)(to_codes + dst * BLOCK);
+    constexpr int N = BLOCK / 16 / THREADS;
+    uint4 x[N];
 #pragma unroll
-    for (int i = 0; i < (int)(BLOCK / 16); i += THREADS) to[i + t] = from[i + t];
+    for (int i = 0; i < N; ++i) x[i] = gload_u4(codes + src * BLOCK + (size_t)(i * THREADS + t) * 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i) *(uint4*)(to_codes + dst * BLOCK + (size_t)(i * THREADS + t) * 16) = x[i];
     if (t == 0) to_scales[dst] = scales[src];
 }
 
@@ -335,6 +411,11 @@ struct HostRows {
 void check_sequences(const char* what, const void* sequences, const void* counts, int n) {
     if (n < 0) fail(std::string(what) + ": a negative number of sequences");
     if (n && (!sequences || !counts)) fail(std::string(what) + ": sequences or rows is NULL");
+}
+
+// Whether 4 dims of any row and head are 16 bytes at a 16-byte address.
+bool vectors(int hd, const void* k, int64_t ks, const void* v, int64_t vs) {
+    return hd % 4 == 0 && ks % 4 == 0 && vs % 4 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
 }
 
 // The sum of n row counts, each 0 or more.
@@ -542,7 +623,8 @@ int trit_hip_paged_append_device(TritHipPagedCache* cache, int layer, const int3
             if (!most) continue;
             auto kernel = cache->hdp == 64 ? append_kernel<64> : append_kernel<128>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)most, (unsigned)cache->kv_heads, (unsigned)(2 * m)), dim3(THREADS),
-                               0, s, cache->pool(layer), a, k, (long long)k_stride, v, (long long)v_stride);
+                               0, s, cache->pool(layer), a, k, (long long)k_stride, v, (long long)v_stride,
+                               vectors(cache->hd, k, k_stride, v, v_stride));
             TRIT_HIP(hipGetLastError());
         }
         return 0;
@@ -606,7 +688,8 @@ int trit_hip_paged_read_device(TritHipPagedCache* cache, int layer, const int32_
             if (!most) continue;
             auto kernel = cache->hdp == 64 ? read_kernel<64> : read_kernel<128>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)most, (unsigned)cache->kv_heads, (unsigned)(2 * m)), dim3(THREADS),
-                               0, s, cache->pool(layer), a, k, (long long)k_stride, v, (long long)v_stride);
+                               0, s, cache->pool(layer), a, k, (long long)k_stride, v, (long long)v_stride,
+                               vectors(cache->hd, k, k_stride, v, v_stride));
             TRIT_HIP(hipGetLastError());
         }
         return 0;

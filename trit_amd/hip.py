@@ -750,6 +750,16 @@ def _ids(values):
     return np.ascontiguousarray(np.asarray(values, dtype=np.int32).reshape(-1))
 
 
+_CHAR, _ADDRESS = C.c_char.from_buffer, C.addressof
+
+
+def _at(a):
+    """The address of an int32 array (in a quarter of a microsecond; `a.ctypes` takes one to two)."""
+    if not a.size:
+        return None
+    return _ADDRESS(_CHAR(a)) if a.flags.writeable else a.ctypes.data
+
+
 def _counts(ids, counts, what):
     counts = _ids(counts)
     if counts.size != ids.size:
@@ -783,24 +793,24 @@ class PagedCache:
     def fork(self, sequences, stream=None):
         ids = _ids(sequences)
         out = np.empty(ids.size, np.int32)
-        check(lib().trit_hip_paged_fork(self.h, ptr(ids), ids.size, ptr(out), stream))
+        check(lib().trit_hip_paged_fork(self.h, _at(ids), ids.size, ptr(out), stream))
         return out
 
     def reorder(self, sequences, parents, stream=None):
         ids = _ids(sequences)
         parents = _counts(ids, parents, "paged reorder")
-        check(lib().trit_hip_paged_reorder(self.h, ptr(ids), ptr(parents), ids.size, stream))
+        check(lib().trit_hip_paged_reorder(self.h, _at(ids), _at(parents), ids.size, stream))
 
     def copy(self, sequences, into=None, stream=None):
         ids = _ids(sequences)
         out = np.empty(ids.size, np.int32)
-        check(lib().trit_hip_paged_copy(self.h, ptr(ids), ids.size, into.h if into is not None else None, ptr(out),
+        check(lib().trit_hip_paged_copy(self.h, _at(ids), ids.size, into.h if into is not None else None, ptr(out),
                                         stream))
         return out
 
     def close(self, sequences):
         ids = _ids(sequences)
-        check(lib().trit_hip_paged_close(self.h, ptr(ids), ids.size))
+        check(lib().trit_hip_paged_close(self.h, _at(ids), ids.size))
 
     def compact(self, stream=None):
         return check(lib().trit_hip_paged_compact(self.h, stream))
@@ -829,12 +839,12 @@ class PagedCache:
         total, width = int(rows.sum()), self.kv_heads * self.head_dim
         k = self._host_rows(k, total, width, "paged append")
         v = self._host_rows(v, total, width, "paged append")
-        check(lib().trit_hip_paged_append(self.h, layer, ptr(ids), ptr(rows), ids.size, ptr(k), ptr(v)))
+        check(lib().trit_hip_paged_append(self.h, layer, _at(ids), _at(rows), ids.size, ptr(k), ptr(v)))
 
     def append_device(self, layer, sequences, rows, k, k_stride, v, v_stride, stream=None):
         ids = _ids(sequences)
         rows = _counts(ids, rows, "paged append")
-        check(lib().trit_hip_paged_append_device(self.h, layer, ptr(ids), ptr(rows), ids.size, k, k_stride, v, v_stride,
+        check(lib().trit_hip_paged_append_device(self.h, layer, _at(ids), _at(rows), ids.size, k, k_stride, v, v_stride,
                                                  stream))
 
     def read(self, layer, sequences, first, rows):
@@ -843,13 +853,13 @@ class PagedCache:
         first, rows = _counts(ids, first, "paged read"), _counts(ids, rows, "paged read")
         shape = (max(int(rows.sum()), 0), self.kv_heads * self.head_dim)
         k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
-        check(lib().trit_hip_paged_read(self.h, layer, ptr(ids), ptr(first), ptr(rows), ids.size, ptr(k), ptr(v)))
+        check(lib().trit_hip_paged_read(self.h, layer, _at(ids), _at(first), _at(rows), ids.size, ptr(k), ptr(v)))
         return k, v
 
     def read_device(self, layer, sequences, first, rows, k, k_stride, v, v_stride, stream=None):
         ids = _ids(sequences)
         first, rows = _counts(ids, first, "paged read"), _counts(ids, rows, "paged read")
-        check(lib().trit_hip_paged_read_device(self.h, layer, ptr(ids), ptr(first), ptr(rows), ids.size, k, k_stride, v,
+        check(lib().trit_hip_paged_read_device(self.h, layer, _at(ids), _at(first), _at(rows), ids.size, k, k_stride, v,
                                                v_stride, stream))
 
     def attention(self, layer, sequences, rows, q, heads, scale=0.0):
@@ -859,14 +869,14 @@ class PagedCache:
         total, width = int(rows.sum()), heads * self.head_dim
         q = self._host_rows(q, total, width, "paged attention")
         out = np.empty((max(total, 0), max(width, 0)), np.float32)
-        check(lib().trit_hip_paged_attention(self.h, layer, ptr(ids), ptr(rows), ids.size, ptr(q), heads, scale,
+        check(lib().trit_hip_paged_attention(self.h, layer, _at(ids), _at(rows), ids.size, ptr(q), heads, scale,
                                              ptr(out)))
         return out
 
     def attention_device(self, layer, sequences, rows, q, q_stride, heads, out, scale=0.0, stream=None):
         ids = _ids(sequences)
         rows = _counts(ids, rows, "paged attention")
-        check(lib().trit_hip_paged_attention_device(self.h, layer, ptr(ids), ptr(rows), ids.size, q, q_stride, heads,
+        check(lib().trit_hip_paged_attention_device(self.h, layer, _at(ids), _at(rows), ids.size, q, q_stride, heads,
                                                     scale, out, stream))
 
     def free(self):
@@ -901,12 +911,12 @@ class CrossStates:
         k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
         if k.size != total * width or v.size != total * width:
             raise TritError(f"cross set: {k.size} and {v.size} values where {total} rows of {width} are needed")
-        check(lib().trit_hip_cross_set(self.h, layer, ptr(slots), ptr(keys), slots.size, ptr(k), ptr(v)))
+        check(lib().trit_hip_cross_set(self.h, layer, _at(slots), _at(keys), slots.size, ptr(k), ptr(v)))
 
     def set_device(self, layer, slots, keys, k, k_stride, v, v_stride, stream=None):
         slots = _ids(slots)
         keys = _counts(slots, keys, "cross set")
-        check(lib().trit_hip_cross_set_device(self.h, layer, ptr(slots), ptr(keys), slots.size, k, k_stride, v, v_stride,
+        check(lib().trit_hip_cross_set_device(self.h, layer, _at(slots), _at(keys), slots.size, k, k_stride, v, v_stride,
                                               stream))
 
     def keys(self, slot, layer=0):
@@ -921,14 +931,14 @@ class CrossStates:
         if q.size != total * width:
             raise TritError(f"cross attention: {q.size} values where {total} rows of {width} are needed")
         out = np.empty((max(total, 0), max(width, 0)), np.float32)
-        check(lib().trit_hip_cross_attention(self.h, layer, ptr(slots), ptr(rows), slots.size, ptr(q), heads, scale,
+        check(lib().trit_hip_cross_attention(self.h, layer, _at(slots), _at(rows), slots.size, ptr(q), heads, scale,
                                              ptr(out)))
         return out
 
     def attention_device(self, layer, slots, rows, q, q_stride, heads, out, scale=0.0, stream=None):
         slots = _ids(slots)
         rows = _counts(slots, rows, "cross attention")
-        check(lib().trit_hip_cross_attention_device(self.h, layer, ptr(slots), ptr(rows), slots.size, q, q_stride, heads,
+        check(lib().trit_hip_cross_attention_device(self.h, layer, _at(slots), _at(rows), slots.size, q, q_stride, heads,
                                                     scale, out, stream))
 
     def free(self):
