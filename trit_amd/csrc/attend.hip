@@ -1,5 +1,6 @@
 // Attention of a few or many query rows to int8 blocks (a paged cache's full
 // ones) and f16 blocks (its open ones, or an encoder's states).
+#include <algorithm>
 #include <climits>
 
 #include "attend.h"
@@ -13,7 +14,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int WAVES = 4;
+// Chunks that a tile's keys are split into at most.
+constexpr int MOST_CHUNKS = 128;
 // The largest fixed-point value of three int8 digits, and the factor that
 // keeps the low part of an f16 pair clear of subnormal f16.
 constexpr float FIXED = 8323072.0f;  // 127 * 65536
@@ -395,7 +397,7 @@ __device__ __forceinline__ float2 get(const float* p) {
 // The four waves take the chunk's blocks in turn and join their sums in shared
 // memory. Of the workgroups of a tile's chunks the last to end joins theirs,
 // in the chunks' order.
-template <int HDP, bool PAGED>
+template <int HDP, bool PAGED, int WAVES>
 __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     constexpr int NT = HDP / 16, KS = HDP / 64, PS = HDP + 4;
     constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
@@ -407,9 +409,10 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     const int w = __builtin_amdgcn_readfirstlane(t / WAVE);
     // The last sequence whose items start at or before this one (the starts behind the last are past every item).
     const int g = blockIdx.x;
-    int si = 0;
+    int si = a.n == 1;
+    if (!si)
 #pragma unroll
-    for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
+        for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
     const AttendSeq seq = a.s[si - 1];
     const int item = (int)blockIdx.y - seq.start;
     const int tile = seq.chunks == 1 ? item : item / seq.chunks, chunk = item - tile * seq.chunks;
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
 
     // The thread's query values are on their way while the first keys are.
     float qv[NT];
-    {
+    if (t < 256) {
         const int c = t / 16, r = row_of(c), h = g * a.group + rest + c - r * a.group;
         const bool valid = c < cols;
         load_queries<HDP, PAGED>(valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q, valid,
@@ -455,7 +458,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024);
             page = b + WAVES < last ? table[b + WAVES] : 0;
         }
-        put_queries<HDP, PAGED>(qv, qs);
+        if (t < 256) put_queries<HDP, PAGED>(qv, qs);
         __syncthreads();
         v4i qd[3][KS];
 #pragma unroll
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             load(kf, b, 0);
             if (AHEAD) load(vf, b, 1);
         }
-        put_queries<HDP, PAGED>(qv, qs);
+        if (t < 256) put_queries<HDP, PAGED>(qv, qs);
         __syncthreads();
         const float step = qs.top[col] * (LOG2E / PAIR);
         for (; b < end; b += WAVES) {
@@ -594,38 +597,36 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     }
     __syncthreads();
     if (!arrived) return;
-    // Chunk v's item; wave w joins the chunks w, w + 4, .. of each column, lane l their elements 2 l, 2 l + 1.
+    // The chunks' largest scores and sums, then their outputs: a thread two dims of a column, its loads all in flight.
     const size_t first = (size_t)(seq.start + tile * seq.chunks) * a.kv_heads + g;
-    for (int cc = 0; cc < cols; ++cc) {
-        float m = -INFINITY, l = 0.0f;
-        float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-        for (int v = w; v < seq.chunks; v += WAVES) {
-            const size_t at = (first + (size_t)v * a.kv_heads) * 16 + cc;
-            const float2 ml = get((const float*)(a.tops + at));
-            const float2 x = 2 * lane < HDP ? get(a.sums + at * HDP + 2 * lane) : make_float2(0.0f, 0.0f);
-            const float mn = __builtin_fmaxf(m, ml.x);
-            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            const float h = ml.x == mn ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-            l = __builtin_fmaf(ml.y, h, l * f);
-            o.x = __builtin_fmaf(x.x, h, o.x * f);
-            o.y = __builtin_fmaf(x.y, h, o.y * f);
-            m = mn;
-        }
-        if (lane == 0) {
-            top[w][cc] = m;
-            sum[w][cc] = l;
-        }
-        if (2 * lane < HDP) {
-            part[w][cc][2 * lane] = o.x;
-            part[w][cc][2 * lane + 1] = o.y;
-        }
+    float* tops = &part[0][0][0];
+    float* sums = tops + 16 * MOST_CHUNKS;
+    static_assert(sizeof(part) >= 2 * 16 * MOST_CHUNKS * sizeof(float), "a chunk's entries fit the waves' parts");
+    for (int i = t; i < cols * seq.chunks; i += WAVES * WAVE) {
+        const int cc = i / seq.chunks, v = i - cc * seq.chunks;
+        const float2 ml = get((const float*)(a.tops + (first + (size_t)v * a.kv_heads) * 16 + cc));
+        tops[i] = ml.x;
+        sums[i] = ml.y;
     }
     __syncthreads();
-    for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
-        float m, l;
-        const float o = joined(i / HDP, i % HDP, m, l);
-        store(i / HDP, i % HDP, o, l);
+    constexpr int PAIRS = HDP / 2;
+    for (int i = t; i < cols * PAIRS; i += WAVES * WAVE) {
+        const int cc = i / PAIRS, e = i % PAIRS * 2;
+        const float* m = tops + cc * seq.chunks;
+        float most = m[0];
+        for (int v = 1; v < seq.chunks; ++v) most = __builtin_fmaxf(most, m[v]);
+        float l = 0.0f;
+        float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll 16
+        for (int v = 0; v < seq.chunks; ++v) {
+            const float2 x = get(a.sums + ((first + (size_t)v * a.kv_heads) * 16 + cc) * HDP + e);
+            const float f = m[v] == most ? 1.0f : __builtin_amdgcn_exp2f(m[v] - most);
+            l = __builtin_fmaf(sums[cc * seq.chunks + v], f, l);
+            o.x = __builtin_fmaf(x.x, f, o.x);
+            o.y = __builtin_fmaf(x.y, f, o.y);
+        }
+        store(cc, e, o.x, l);
+        store(cc, e + 1, o.y, l);
     }
 }
 
@@ -635,6 +636,8 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
 // most workgroups where keys are split: what the scratch holds.
 constexpr long long MOST_TILES = 65535;
 constexpr long long SPLIT_ITEMS = 1024;
+// Workgroups of 8 waves that the compute units take at once.
+constexpr long long FEW_ITEMS = 256;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
     memory.alloc(SPLIT_ITEMS * (16 * ((size_t)hdp * 4 + 8) + 4));
@@ -655,6 +658,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     for (size_t from = 0; from < seqs.size();) {
         // The launch's sequences, and its work in blocks of keys.
         long long whole = 0, work = 0;
+        int most = 0;
         size_t to = from;
         for (a.n = 0; to < seqs.size() && a.n < CALL_SEQS; ++to) {
             if (seqs[to].rows == 0) continue;
@@ -662,15 +666,30 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
             if (a.n && whole + tiles(seqs[to]) > MOST_TILES) break;
             whole += tiles(seqs[to]);
             work += tiles(seqs[to]) * blocks(seqs[to]);
+            most = std::max(most, blocks(seqs[to]));
             a.s[a.n++] = seqs[to];
         }
         from = to;
         if (!a.n) return;
-        // Chunks of as few blocks as keep the items within the scratch, a multiple of what the waves take at once.
+        // Where 8-wave workgroups leave compute units free, latency is what counts: 8 waves with two rounds and no
+        // join up to 16 blocks, one round a chunk above. One token of 700, 16/8 heads of 128: 8.1 us (4 waves a
+        // chunk: 8.4); 5 rows over 1500 states, 20 heads of 64: 8.0 (8.8). Else 4 waves and chunks of as few
+        // blocks as keep the items within the scratch, a multiple of what the waves take at once: 32 requests of
+        // 100 to 8001 tokens 33.5 us (8 waves: 36.9), two of 131 K 105 (112).
+        long long small = 0;
+        for (int i = 0; i < a.n; ++i) {
+            const long long nb = blocks(a.s[i]);
+            small += tiles(a.s[i]) * (nb <= 16 ? 1 : (nb + 7) / 8);
+        }
+        const int waves = small * a.kv_heads <= FEW_ITEMS ? 8 : 4;
         a.chunk = INT_MAX / 2;
         const long long room = SPLIT_ITEMS / a.kv_heads - whole;
-        if (room > 0) a.chunk = (int)((work + room - 1) / room + WAVES - 1) / WAVES * WAVES;
-        if (a.chunk < WAVES) a.chunk = WAVES;
+        if (waves == 8) {
+            a.chunk = std::max(most <= 16 ? 16 : 8, (most + MOST_CHUNKS - 1) / MOST_CHUNKS);
+        } else if (room > 0) {
+            const long long least = std::max({(work + room - 1) / room, (long long)(most + MOST_CHUNKS - 1) / MOST_CHUNKS, 1LL});
+            a.chunk = (int)((least + waves - 1) / waves * waves);
+        }
         int items = 0, groups = 0;
         for (int i = 0; i < CALL_SEQS; ++i) {
             AttendSeq& q = a.s[i];
@@ -685,18 +704,12 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
             items += (int)tiles(q) * q.chunks;
             if (q.chunks > 1) groups += (int)tiles(q);
         }
-        const dim3 grid((unsigned)a.kv_heads, (unsigned)items), block(WAVES * WAVE);
-        if (hdp == 64) {
-            if (paged)
-                hipLaunchKernelGGL((attend_kernel<64, true>), grid, block, 0, s, a);
-            else
-                hipLaunchKernelGGL((attend_kernel<64, false>), grid, block, 0, s, a);
-        } else {
-            if (paged)
-                hipLaunchKernelGGL((attend_kernel<128, true>), grid, block, 0, s, a);
-            else
-                hipLaunchKernelGGL((attend_kernel<128, false>), grid, block, 0, s, a);
-        }
+        const dim3 grid((unsigned)a.kv_heads, (unsigned)items), block((unsigned)(waves * WAVE));
+        auto kernel = hdp == 64 ? (paged ? (waves == 4 ? attend_kernel<64, true, 4> : attend_kernel<64, true, 8>)
+                                         : (waves == 4 ? attend_kernel<64, false, 4> : attend_kernel<64, false, 8>))
+                                : (paged ? (waves == 4 ? attend_kernel<128, true, 4> : attend_kernel<128, true, 8>)
+                                         : (waves == 4 ? attend_kernel<128, false, 4> : attend_kernel<128, false, 8>));
+        hipLaunchKernelGGL(kernel, grid, block, 0, s, a);
         TRIT_HIP(hipGetLastError());
     }
 }
