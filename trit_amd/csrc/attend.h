@@ -42,9 +42,10 @@ struct AttendSeq {
     int len;    // keys
     int rows;   // query rows
     int first;  // its first row in q and out
-    // Set by attend(): its first item of the launch, its first group of items
-    // that are joined, the items its keys are split into.
-    int start, group, chunks;
+    // Set by attend(): its first item of the launch; its first group of items
+    // that are joined, and its first item among those; the items its keys are
+    // split into.
+    int start, group, part, chunks;
 };
 
 // Device memory of a handle for keys that are split over workgroups: each

@@ -203,7 +203,10 @@ __device__ __forceinline__ void pin(float& a, float& b, float& c, float& d) {
     asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
 }
 
-__device__ __forceinline__ v4i load16(const uint8_t* p) { return *(const TRIT_GLOBAL v4i*)p; }
+// 16 bytes of a lane at a wave's address (in scalar registers) and the lane's offset.
+__device__ __forceinline__ v4i load16(const uint8_t* wave, uint32_t lane) {
+    return *(const TRIT_GLOBAL v4i*)((const TRIT_GLOBAL uint8_t*)wave + lane);
+}
 
 // A full block of int8 codes, its keys' and values' fragments in registers.
 // Both products run in integers: the query and the probabilities are three
@@ -268,7 +271,9 @@ __device__ __forceinline__ bool any_nan(v8h x) {
     return hit != 0;
 }
 
-__device__ __forceinline__ v8h load8h(const _Float16* p) { return *(const TRIT_GLOBAL v8h*)p; }
+__device__ __forceinline__ v8h load8h(const _Float16* wave, uint32_t lane) {
+    return *(const TRIT_GLOBAL v8h*)((const TRIT_GLOBAL uint8_t*)wave + lane);
+}
 
 // An f16 block, the queries (from shared memory) and probabilities as f16 pairs.
 template <int HDP>
@@ -440,6 +445,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     Running<HDP> run;
     run.clear();
     int b = b0 + w;
+    const uint32_t lane16 = lane * 16;
     if constexpr (PAGED) {
         const int full = seq.len / BLOCK_TOKENS;  // full blocks hold codes
         const int last = end < full ? end : full;
@@ -450,12 +456,12 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         const uint8_t* block = nullptr;
         if (b < last) {
             const size_t at = (size_t)page * a.kv_heads + g;
-            block = a.codes + at * BLOCK + lane * 16;
+            block = a.codes + at * BLOCK;
             sc = a.scales[at];
 #pragma unroll
-            for (int i = 0; i < NT; ++i) kf[i] = load16(block + i * 1024);
+            for (int i = 0; i < NT; ++i) kf[i] = load16(block + i * 1024, lane16);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024);
+            for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024, lane16);
             page = b + WAVES < last ? table[b + WAVES] : 0;
         }
         if (t < 256) put_queries<HDP, PAGED>(qv, qs);
@@ -464,7 +470,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qd[j][ks] = *(const v4i*)(qs.digits[j] + ks * 1024 + lane * 16);
+            for (int ks = 0; ks < KS; ++ks) qd[j][ks] = *(const v4i*)(qs.digits[j] + ks * 1024 + lane16);
         const float step = qs.top[col] * (LOG2E / FIXED);
         for (; b < last; b += WAVES) {
             float u[16];
@@ -474,11 +480,11 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             const uint8_t* next = block;
             if (more) {
                 const size_t at = (size_t)page * a.kv_heads + g;
-                next = a.codes + at * BLOCK + lane * 16;
+                next = a.codes + at * BLOCK;
                 sc = a.scales[at];
                 page = b + 2 * WAVES < last ? table[b + 2 * WAVES] : 0;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024);
+                for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024, lane16);
             }
             const float now =
                 block_softmax<HDP>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > ahead, seen - b * BLOCK_TOKENS, run);
@@ -487,33 +493,33 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             if (more) {
                 block = next;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024);
+                for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024, lane16);
             }
         }
         if (b < end) {
-            const _Float16* open = a.f16 + ((size_t)seq.place * a.kv_heads + g) * BLOCK + lane * 8;
+            const _Float16* open = a.f16 + ((size_t)seq.place * a.kv_heads + g) * BLOCK;
             v8h k16[2 * NT], v16[2 * NT];
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) k16[i] = load8h(open + i * 512);
+            for (int i = 0; i < 2 * NT; ++i) k16[i] = load8h(open + i * 512, lane16);
             float u[16];
             const int tokens = seq.len - b * BLOCK_TOKENS, sees = seen - b * BLOCK_TOKENS;
             f16_scores<HDP>(k16, qs.pairs[0], qs.pairs[1], u);
             // (With the values' loads before the scores' products the 128-wide kernel spills.)
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) v16[i] = load8h(open + BLOCK / 2 + i * 512);
+            for (int i = 0; i < 2 * NT; ++i) v16[i] = load8h(open + BLOCK / 2 + i * 512, lane16);
             const float now = block_softmax<HDP>(u, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
             open_values<HDP>(v16, u, now, tokens, sees, run);
         }
     } else {
         const _Float16* states =
-            a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * BLOCK + lane * 8;
+            a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * BLOCK;
         // 64 wide, the next block's values are on their way too; 128 wide they would not fit the registers.
         constexpr bool AHEAD = HDP == 64;
         v8h kf[2 * NT], vf[2 * NT];
         auto load = [&](v8h(&f)[2 * NT], int at, int half) {
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) f[i] = load8h(states + at * BLOCK + half * (BLOCK / 2) + i * 512);
+            for (int i = 0; i < 2 * NT; ++i) f[i] = load8h(states + at * BLOCK + half * (BLOCK / 2) + i * 512, lane16);
         };
         if (b < end) {
             load(kf, b, 0);
@@ -582,7 +588,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         const int cc = i / HDP, e = i % HDP;
         float m, l;
         const float o = joined(cc, e, m, l);
-        const size_t at = ((size_t)blockIdx.y * a.kv_heads + g) * 16 + cc;
+        const size_t at = ((size_t)(seq.part + item) * a.kv_heads + g) * 16 + cc;
         put(a.sums + at * HDP + e, o);
         if (e == 0) put(a.tops + at, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(m));
     }
@@ -598,7 +604,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     __syncthreads();
     if (!arrived) return;
     // The chunks' largest scores and sums, then their outputs: a thread two dims of a column, its loads all in flight.
-    const size_t first = (size_t)(seq.start + tile * seq.chunks) * a.kv_heads + g;
+    const size_t first = (size_t)(seq.part + tile * seq.chunks) * a.kv_heads + g;
     float* tops = &part[0][0][0];
     float* sums = tops + 16 * MOST_CHUNKS;
     static_assert(sizeof(part) >= 2 * 16 * MOST_CHUNKS * sizeof(float), "a chunk's entries fit the waves' parts");
@@ -632,9 +638,9 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
 
 }  // namespace
 
-// Tiles of one launch (65535 blocks in the grid's second dimension), and the
-// most workgroups where keys are split: what the scratch holds.
-constexpr long long MOST_TILES = 65535;
+// Tiles of one launch (the grid's second dimension), and the most workgroups
+// of split keys: what the scratch holds.
+constexpr long long MOST_TILES = 50000;
 constexpr long long SPLIT_ITEMS = 1024;
 // Workgroups of 8 waves that the compute units take at once.
 constexpr long long FEW_ITEMS = 256;
@@ -673,36 +679,52 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
         if (!a.n) return;
         // Where 8-wave workgroups leave compute units free, latency is what counts: 8 waves with two rounds and no
         // join up to 16 blocks, one round a chunk above. One token of 700, 16/8 heads of 128: 8.1 us (4 waves a
-        // chunk: 8.4); 5 rows over 1500 states, 20 heads of 64: 8.0 (8.8). Else 4 waves and chunks of as few
-        // blocks as keep the items within the scratch, a multiple of what the waves take at once: 32 requests of
-        // 100 to 8001 tokens 33.5 us (8 waves: 36.9), two of 131 K 105 (112).
+        // chunk: 8.4); 5 rows over 1500 states, 20 heads of 64: 8.0 (8.8). Else 4 waves, and chunks of two rounds
+        // or more: as few as make no more than two workgroups a compute unit, which is what they hold, or a quarter
+        // more than there are without a split. 32 requests of 100 to 8001 tokens: 33.1 us with 512 workgroups,
+        // 35.3 with 760, 41 with 2030; two of 131 K 101 us with 512, 105 with 1024, 112 with 8 waves.
         long long small = 0;
         for (int i = 0; i < a.n; ++i) {
             const long long nb = blocks(a.s[i]);
             small += tiles(a.s[i]) * (nb <= 16 ? 1 : (nb + 7) / 8);
         }
         const int waves = small * a.kv_heads <= FEW_ITEMS ? 8 : 4;
-        a.chunk = INT_MAX / 2;
-        const long long room = SPLIT_ITEMS / a.kv_heads - whole;
+        long long split = 0;  // items of split sequences
+        const auto items_of = [&](int chunk) {
+            long long all = split = 0;
+            for (int i = 0; i < a.n; ++i) {
+                const long long c = std::max((blocks(a.s[i]) + chunk - 1) / chunk, 1), t = tiles(a.s[i]) * c;
+                all += t;
+                if (c > 1) split += t;
+            }
+            return all;
+        };
         if (waves == 8) {
             a.chunk = std::max(most <= 16 ? 16 : 8, (most + MOST_CHUNKS - 1) / MOST_CHUNKS);
-        } else if (room > 0) {
-            const long long least = std::max({(work + room - 1) / room, (long long)(most + MOST_CHUNKS - 1) / MOST_CHUNKS, 1LL});
-            a.chunk = (int)((least + waves - 1) / waves * waves);
+            items_of(a.chunk);
+        } else {
+            const long long room = std::max(2 * FEW_ITEMS / a.kv_heads, whole + whole / 4);
+            a.chunk = (int)std::max({work / room, (long long)(most + MOST_CHUNKS - 1) / MOST_CHUNKS, 2LL * waves});
+            a.chunk = (a.chunk + waves - 1) / waves * waves;
+            while (items_of(a.chunk) > room || split * a.kv_heads > SPLIT_ITEMS)
+                a.chunk += (a.chunk / 8 + waves) / waves * waves;
         }
-        int items = 0, groups = 0;
+        int items = 0, groups = 0, parts = 0;
         for (int i = 0; i < CALL_SEQS; ++i) {
             AttendSeq& q = a.s[i];
             if (i >= a.n) {
                 q.start = INT_MAX;
                 continue;
             }
-            const int nb = blocks(q);
-            q.chunks = nb <= a.chunk ? 1 : (nb + a.chunk - 1) / a.chunk;
+            q.chunks = std::max((blocks(q) + a.chunk - 1) / a.chunk, 1);
             q.start = items;
             q.group = groups;
+            q.part = parts;
             items += (int)tiles(q) * q.chunks;
-            if (q.chunks > 1) groups += (int)tiles(q);
+            if (q.chunks > 1) {
+                groups += (int)tiles(q);
+                parts += (int)tiles(q) * q.chunks;
+            }
         }
         const dim3 grid((unsigned)a.kv_heads, (unsigned)items), block((unsigned)(waves * WAVE));
         auto kernel = hdp == 64 ? (paged ? (waves == 4 ? attend_kernel<64, true, 4> : attend_kernel<64, true, 8>)

@@ -245,7 +245,7 @@ int trit_hip_cross_attention_device(TritHipCross* cross, int layer, const int32_
             if (keys < 0)
                 fail("cross attention: slot " + std::to_string(slots[i]) + " of layer " + std::to_string(layer) +
                      " was never set");
-            seqs.push_back({slots[i], keys, rows[i], first, 0, 0, 0});
+            seqs.push_back({slots[i], keys, rows[i], first, 0, 0, 0, 0});
             first += rows[i];
         }
         const hipStream_t s = cross->enter(stream_);

@@ -738,7 +738,7 @@ int trit_hip_paged_attention_device(TritHipPagedCache* cache, int layer, const i
             if (rows[i] > len)
                 fail("paged attention: " + std::to_string(rows[i]) + " query rows of sequence " +
                      std::to_string(sequences[i]) + ", which holds " + std::to_string(len) + " tokens");
-            seqs.push_back({cache->book.row(sequences[i]), len, rows[i], first, 0, 0, 0});
+            seqs.push_back({cache->book.row(sequences[i]), len, rows[i], first, 0, 0, 0, 0});
             first += rows[i];
         }
         const hipStream_t s = cache->enter(stream_);
