@@ -19,7 +19,7 @@ constexpr int MOST_CHUNKS = 128;
 // The largest fixed-point value of three int8 digits, and the factor that
 // keeps the low part of an f16 pair clear of subnormal f16.
 constexpr float FIXED = 8323072.0f;  // 127 * 65536
-constexpr float PAIR = 1024.0f;
+constexpr float PAIR = 1024.0f, LOG_PAIR = 10.0f;
 
 // The larger of a value and the one 32 (16) lanes away: a swap of two copies
 // leaves a lane its own value in one and the other's in the other.
@@ -636,6 +636,333 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     }
 }
 
+// ---- many rows -------------------------------------------------------------
+
+// The f16 pairs hi + lo of two values. (The factor -1 comes in a register the
+// compiler does not know the value of: it makes one mixed-precision
+// multiply-add of each rest, a conversion and a subtraction otherwise.)
+__device__ __forceinline__ void split2(float a, float b, float minus_one, uint32_t& hi, uint32_t& lo) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    h2 h = {(_Float16)a, (_Float16)b};
+    uint32_t bits = __builtin_bit_cast(uint32_t, h);
+    asm("" : "+v"(bits));
+    h = __builtin_bit_cast(h2, bits);
+    const h2 l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, a), (_Float16)__builtin_fmaf((float)h[1], minus_one, b)};
+    hi = bits;
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// Four int8 codes as f16, exactly: the byte c + 128 below an exponent of 2^10 is 1152 + c.
+__device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& h01, uint32_t& h23) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const uint32_t u = c ^ 0x80808080u;
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+    const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+    h01 = __builtin_bit_cast(uint32_t, a);
+    h23 = __builtin_bit_cast(uint32_t, b);
+}
+
+// Attention where a sequence has many query columns: workgroup (g, item) takes
+// 64 columns of a sequence (column r * group + c: row r, head g * group + c),
+// a wave 16 of them over every key block they see. The blocks pass through
+// shared memory as f16 fragments, once for the four waves, the next one's
+// loads in flight while one is worked on; int8 codes are widened on the way
+// (exactly), so both products run on f16 pairs of the queries and
+// probabilities. Against the integer form above, whose three digits need
+// 420 vector instructions a block and 16 columns, this takes 230, and those
+// are what binds; the columns of later rows start first (they see the most).
+// A probability is a pair relative to the running maximum, times PAIR: what
+// is lost of it is below 2^-34 of the largest.
+template <int HDP, bool PAGED>
+__global__ __launch_bounds__(256, HDP == 128 ? 2 : PAGED ? 3 : 4) void attend_rows_kernel(AttendArgs a) {
+    constexpr int NT = HDP / 16, KS = HDP / 32, F = BLOCK_TOKENS * HDP * 2 / 8 / 256;  // 16-byte pieces a thread
+    constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
+    __shared__ __align__(16) _Float16 kv[2][BLOCK];
+    const int t = threadIdx.x, lane = t % WAVE, col = lane % 16, lq = lane / 16;
+    const int w = __builtin_amdgcn_readfirstlane(t / WAVE);
+    const int g = blockIdx.x;
+    int si = a.n == 1;
+    if (!si)
+#pragma unroll
+        for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
+    const AttendSeq seq = a.s[si - 1];
+    const int columns = seq.rows * a.group;
+    const int wide = (columns + 63) / 64 - 1 - ((int)blockIdx.y - seq.start);  // 64 columns, the last ones first
+    const int tile = wide * 4 + w, cols = min(columns - tile * 16, 16);  // may be 0 or less: a wave without columns
+    const int row0 = tile * 16 / a.group, rest = tile * 16 - row0 * a.group;
+    const int r = (int)(((float)(rest + col) + 0.5f) * (1.0f / (float)a.group)), h = g * a.group + rest + col - r * a.group;
+    const bool valid = col < cols;
+    // Keys: what the lane's column sees, the least of the wave's columns, the most of the workgroup's.
+    const int ahead = PAGED ? seq.len - seq.rows + 1 : seq.len;
+    const int seen = valid ? ahead + (PAGED ? row0 + r : 0) : 0;
+    const int least = PAGED ? ahead + row0 : ahead;
+    const int most = PAGED ? ahead + (min(wide * 64 + 63, columns - 1)) / a.group : ahead;
+    const int end = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+    const int full = PAGED ? seq.len / BLOCK_TOKENS : 0;
+
+    // The thread's pieces of the next block: codes (4 * F values in F / 2 pieces) or halves.
+    uint4 piece[F];
+    float2 sc = make_float2(1.0f, 1.0f), sn = sc;
+    const int* table = PAGED ? a.table + (size_t)seq.place * a.table_stride : nullptr;
+    auto fetch = [&](int b) {
+        if (PAGED && b < full) {
+            const size_t at = (size_t)table[b] * a.kv_heads + g;
+            const uint8_t* src = a.codes + at * BLOCK;
+            sn = a.scales[at];
+#pragma unroll
+            for (int i = 0; i < F / 2; ++i) piece[i] = gload_u4(src + i * 4096 + t * 16);
+        } else {
+            const _Float16* src = PAGED ? a.f16 + ((size_t)seq.place * a.kv_heads + g) * BLOCK
+                                        : a.f16 + (((size_t)seq.place * a.kv_heads + g) * a.blocks + b) * BLOCK;
+            sn = make_float2(1.0f, 1.0f);
+#pragma unroll
+            for (int i = 0; i < F; ++i) piece[i] = gload_u4(src + i * 2048 + t * 8);
+        }
+    };
+    // Into shared memory as f16 fragments; of an open block, values behind the last token as 0. Returns whether an
+    // open block holds a NaN value.
+    auto put_block = [&](int b, _Float16* to) {
+        bool nan = false;
+        if (PAGED && b < full) {
+#pragma unroll
+            for (int i = 0; i < F / 2; ++i) {
+                const uint32_t c[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
+                uint32_t x[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) codes_to_f16(c[j], x[2 * j], x[2 * j + 1]);
+                // Piece u = 256 i + t of the block: fragment f, its lane l. K: 16 dims of a token, two lanes' worth
+                // of one f16 fragment. V: 16 tokens of a dim, one lane's in each of two fragments.
+                const int f = i * 4 + t / WAVE, l = lane;
+                int at0, at1;
+                if (i < F / 4) {
+                    const int tile16 = f / (HDP / 64), ks = f % (HDP / 64) * 2 + l / 32;
+                    at0 = ((tile16 * KS + ks) * 64 + l / 16 % 2 * 32 + l % 16) * 8;
+                    at1 = at0 + 16 * 8;
+                } else {
+                    at0 = BLOCK / 2 + ((f - NT) * 2 * 64 + l) * 8;
+                    at1 = at0 + 64 * 8;
+                }
+                *(uint4*)(to + at0) = make_uint4(x[0], x[1], x[2], x[3]);
+                *(uint4*)(to + at1) = make_uint4(x[4], x[5], x[6], x[7]);
+            }
+            return nan;
+        }
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            uint4 x = piece[i];
+            if (PAGED && i >= F / 2) {
+                const int s = (i * 4 + t / WAVE) % 2, tokens = seq.len - b * BLOCK_TOKENS;
+                uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int tok = 32 * s + 16 * (j / 2) + 4 * lq + 2 * (j % 2);
+                    y[j] &= tok + 1 < tokens ? 0xffffffffu : tok < tokens ? 0xffffu : 0u;
+                    nan |= (((y[j] & 0x7fff7fffu) + 0x03ff03ffu) & 0x80008000u) != 0;
+                }
+                x = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+            *(uint4*)(to + i * 2048 + t * 8) = x;
+        }
+        return nan;
+    };
+
+    fetch(0);
+    // The lane's query values: dims 32 ks + 8 lq + i of its column, as f16 pairs.
+    v8h qh[KS], ql[KS];
+    float step;
+    {
+        const float* q = valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q;
+        float v[KS][8], top = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int e = 32 * ks + 8 * lq;
+            if (a.aligned) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const float4 x = gload_f4(q + (e + i < a.hd ? e + i : 0));
+                    v[ks][i] = x.x;
+                    v[ks][i + 1] = x.y;
+                    v[ks][i + 2] = x.z;
+                    v[ks][i + 3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[ks][i] = *gmem(q + (e + i < a.hd ? e + i : 0));
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = valid && 32 * ks + 8 * lq + i < a.hd ? v[ks][i] * a.scale : 0.0f;
+                v[ks][i] = x;
+                top = x == x ? __builtin_fmaxf(top, __builtin_fabsf(x)) : INFINITY;
+            }
+        top = column_max(top);
+        const bool finite = top < INFINITY;
+        top = __builtin_fmaxf(top, 1e-30f);
+        const float inv = PAIR / top;
+        step = finite ? top * (LOG2E / PAIR) : NAN;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = finite ? v[ks][i] * inv : 0.0f;
+                qh[ks][i] = (_Float16)x;
+                ql[ks][i] = (_Float16)(x - (float)qh[ks][i]);
+            }
+    }
+    float minus_one = -1.0f;
+    asm("" : "+v"(minus_one));
+    float m = -INFINITY, l = 0.0f;
+    v4f acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+    bool nan = end > 0 && put_block(0, kv[0]);
+    int any_nan_here = __syncthreads_or(PAGED && nan);
+    for (int b = 0; b < end; ++b) {
+        const _Float16* k = kv[b % 2];
+        sc = sn;
+        if (b + 1 < end) fetch(b + 1);
+        if (cols > 0 && (!PAGED || b * BLOCK_TOKENS < ahead + row0 + (rest + cols - 1) / a.group)) {
+            float u[16];
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) {
+                v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const v8h kf = *(const v8h*)(k + (tt * KS + ks) * 512 + lane * 8);
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[ks], c, 0, 0, 0);
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[ks], c, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[4 * tt + i] = c[i];
+            }
+            const float f = step * sc.x;
+            const int sees = seen - b * BLOCK_TOKENS;
+            const bool mask = (b + 1) * BLOCK_TOKENS > least;
+            if (mask) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (16 * (i / 4) + 4 * lq + i % 4 >= sees) u[i] = -INFINITY;
+            }
+            float top = u[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i]);
+            top = column_max(top);
+            // (A column that sees nothing of the block: -inf, also where its scale is 0 or NaN.)
+            const float mn = __builtin_fmaxf(m, top > -INFINITY ? top * f : -INFINITY);
+            const float before = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float ref = mn > -INFINITY ? mn - LOG_PAIR : 0.0f;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[i], f, -ref));
+            if (mask) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (16 * (i / 4) + 4 * lq + i % 4 >= sees) u[i] = 0.0f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += u[i];
+            l = __builtin_fmaf(l, before, sum);
+            if (__any(before != 1.0f)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][i] *= before;
+            }
+            v8h ph[2], pl[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                v4i hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t x, y;
+                    split2(u[8 * s + 2 * i], u[8 * s + 2 * i + 1], minus_one, x, y);
+                    hi[i] = (int)x;
+                    lo[i] = (int)y;
+                }
+                ph[s] = __builtin_bit_cast(v8h, hi);
+                pl[s] = __builtin_bit_cast(v8h, lo);
+            }
+            const _Float16* v = k + BLOCK / 2 + lane * 8;
+            if (PAGED && b < full) {
+                const float sv = sees > 0 ? sc.y : 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const v8h vf = *(const v8h*)(v + (2 * n + s) * 512);
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], c, 0, 0, 0);
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], c, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][i] = __builtin_fmaf(c[i], sv, acc[n][i]);
+                }
+            } else {
+                // As open_values: a NaN value counts for the columns that see its token and no others.
+                if (PAGED && any_nan_here) {
+                    v8h sees16[2];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        sees16[i / 8][i % 8] = (_Float16)(16 * (i / 4) + 4 * lq + i % 4 < sees ? 1.0f : 0.0f);
+                    for (int n = 0; n < NT; ++n) {
+                        v4f count = v4f{0.0f, 0.0f, 0.0f, 0.0f}, c = count;
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            v8h vf = *(const v8h*)(v + (2 * n + s) * 512), is;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const _Float16 x = vf[i];
+                                is[i] = (_Float16)(x != x ? 1.0f : 0.0f);
+                                vf[i] = x != x ? (_Float16)0.0f : x;
+                            }
+                            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees16[s], count, 0, 0, 0);
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], c, 0, 0, 0);
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], c, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int nn = 0; nn < NT; ++nn)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (nn == n) acc[nn][i] += count[i] > 0.0f ? NAN : c[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const v8h vf = *(const v8h*)(v + (2 * n + s) * 512);
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], acc[n], 0, 0, 0);
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], acc[n], 0, 0, 0);
+                        }
+                }
+            }
+        }
+        // The next block goes where the block before this one was: every wave has passed the last barrier.
+        nan = b + 1 < end && put_block(b + 1, kv[(b + 1) % 2]);
+        if (PAGED && b + 1 == full)
+            any_nan_here = __syncthreads_or(nan);
+        else
+            __syncthreads();
+    }
+    l = column_sum(l);
+    if (!valid) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float* out = a.out + ((size_t)(seq.first + row0 + r) * a.kv_heads * a.group + h) * a.hd;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = 16 * n + 4 * lq + i;
+            if (e < a.hd) out[e] = l == 0.0f ? 0.0f : acc[n][i] * inv;
+        }
+}
+
 }  // namespace
 
 // Tiles of one launch (the grid's second dimension), and the most workgroups
@@ -644,6 +971,8 @@ constexpr long long MOST_TILES = 50000;
 constexpr long long SPLIT_ITEMS = 1024;
 // Workgroups of 8 waves that the compute units take at once.
 constexpr long long FEW_ITEMS = 256;
+// Columns of a key head from which the many-row kernel takes a sequence.
+constexpr long long MANY_COLUMNS = 64;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
     memory.alloc(SPLIT_ITEMS * (16 * ((size_t)hdp * 4 + 8) + 4));
@@ -661,19 +990,38 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     const auto tiles = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 15) / 16; };
     const auto blocks = [](const AttendSeq& q) { return (q.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS; };
     a.aligned = a.hd % 4 == 0 && a.qs % 4 == 0 && (uintptr_t)a.q % 16 == 0;
-    for (size_t from = 0; from < seqs.size();) {
+    // Sequences of many columns in launches of their own.
+    std::vector<AttendSeq> few, many;
+    for (const AttendSeq& q : seqs)
+        if (q.rows) ((long long)q.rows * a.group >= MANY_COLUMNS ? many : few).push_back(q);
+    for (size_t at = 0; at < many.size();) {
+        const auto wide = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 63) / 64; };
+        long long items = 0;
+        for (a.n = 0; at < many.size() && a.n < CALL_SEQS; ++at) {
+            AttendSeq q = many[at];
+            if (wide(q) > MOST_TILES) fail("attention: more query rows than one launch takes");
+            if (a.n && items + wide(q) > MOST_TILES) break;
+            q.start = (int)items;
+            items += wide(q);
+            a.s[a.n++] = q;
+        }
+        for (int i = a.n; i < CALL_SEQS; ++i) a.s[i].start = INT_MAX;
+        auto kernel = hdp == 64 ? (paged ? attend_rows_kernel<64, true> : attend_rows_kernel<64, false>)
+                                : (paged ? attend_rows_kernel<128, true> : attend_rows_kernel<128, false>);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.kv_heads, (unsigned)items), dim3(256), 0, s, a);
+        TRIT_HIP(hipGetLastError());
+    }
+    for (size_t from = 0; from < few.size();) {
         // The launch's sequences, and its work in blocks of keys.
         long long whole = 0, work = 0;
         int most = 0;
         size_t to = from;
-        for (a.n = 0; to < seqs.size() && a.n < CALL_SEQS; ++to) {
-            if (seqs[to].rows == 0) continue;
-            if (tiles(seqs[to]) > MOST_TILES) fail("attention: more query rows than one launch takes");
-            if (a.n && whole + tiles(seqs[to]) > MOST_TILES) break;
-            whole += tiles(seqs[to]);
-            work += tiles(seqs[to]) * blocks(seqs[to]);
-            most = std::max(most, blocks(seqs[to]));
-            a.s[a.n++] = seqs[to];
+        for (a.n = 0; to < few.size() && a.n < CALL_SEQS; ++to) {
+            if (a.n && whole + tiles(few[to]) > MOST_TILES) break;
+            whole += tiles(few[to]);
+            work += tiles(few[to]) * blocks(few[to]);
+            most = std::max(most, blocks(few[to]));
+            a.s[a.n++] = few[to];
         }
         from = to;
         if (!a.n) return;
