@@ -50,18 +50,22 @@ def attention(q, k, v, seen, scale):
     group = heads // k.shape[1]
     out, off = np.zeros((rows, heads, hd)), np.zeros((rows, heads, 1))
     e = 2.0 ** -22
-    for r in range(rows):
-        n = int(seen[r])
-        if n == 0:
+    for h in range(heads):
+        kk, vv = k[:, h // group], v[:, h // group]
+        if len(kk) == 0:
             continue
-        for h in range(heads):
-            kk, vv = k[:n, h // group], v[:n, h // group]
-            s = scale * (kk @ q[r, h].astype(np.float64))
+        size = np.abs(kk).sum(axis=1)
+        scores = scale * (q[:, h].astype(np.float64) @ kk.T)
+        for r in range(rows):
+            n = int(seen[r])
+            if n == 0:
+                continue
+            s = scores[r, :n]
             p = np.exp(s - np.max(s))
             # A NaN value counts however small its probability is.
-            out[r, h] = (p / p.sum()) @ vv
-            d = e * scale * np.max(np.abs(q[r, h])) * np.max(np.abs(kk).sum(axis=1)) + 4 * e * np.max(np.abs(s))
-            vmax = np.nanmax(np.abs(vv)) if not np.isnan(vv).all() else 0.0
+            out[r, h] = (p / p.sum()) @ vv[:n]
+            d = e * scale * np.max(np.abs(q[r, h])) * np.max(size[:n]) + 4 * e * np.max(np.abs(s))
+            vmax = np.nanmax(np.abs(vv[:n])) if not np.isnan(vv[:n]).all() else 0.0
             off[r, h] = vmax * (2 * (d + e) + (n / BLOCK + 24) * 2.0 ** -23)
     # Where every key's score is NaN the result is, and the bound says nothing.
     return out, np.nan_to_num(off)

@@ -154,3 +154,66 @@ def test_cross_refusals(gpu):
         fresh.attention(0, [1], [1], x[:1], 2)
     assert [c.keys(0), c.keys(1)] == [10, 20]
     assert c.attention(0, [0], [0], x[:0], 2).shape == (0, 128)
+
+
+def sampled(got, data, slots, rows, heads, q, what):
+    """Some rows of each slot against float64: the ends, tile borders, and others."""
+    hd = q.shape[2]
+    scale = float(np.float32(1.0) / np.sqrt(np.float32(hd)))
+    r = np.random.default_rng(3)
+    at = 0
+    for s, n in zip(slots, rows):
+        pick = sorted({0, n - 1, min(15, n - 1), min(16, n - 1), min(63, n - 1), *r.integers(0, n, 12).tolist()})
+        k, v = (P.f16(x) for x in data[s])
+        idx = at + np.array(pick)
+        want, off = P.attention(q[idx], k, v, [len(k)] * len(pick), scale)
+        near(got[idx], want, off, f"{what} slot {s} of {len(k)} keys, {n} rows")
+        at += n
+
+
+# Calls of many columns a slot, and some of few beside them.
+MANY = [
+    (64, 64, 8, [70, 129, 0], [1, 0, 2], [400, 3, 70]),
+    (128, 32, 4, [65], [0], [900]),
+    (80, 24, 3, [130, 1], [0, 1], [900, 129]),
+    (40, 20, 20, [64, 200], [1, 0, 1], [700, 600, 65]),
+]
+
+
+@pytest.mark.parametrize("hd,heads,kvh,keys,slots,rows", MANY)
+def test_cross_many_rows(gpu, hd, heads, kvh, keys, slots, rows):
+    print(f"case cross many rows hd={hd} heads={heads}/{kvh} keys={keys} rows={rows}", flush=True)
+    c, data = states(hd, kvh, keys)
+    q = queries(61, sum(rows), heads, hd)
+    got = c.attention(0, slots, rows, q, heads).reshape(-1, heads, hd)
+    assert np.isfinite(got).all()
+    sampled(got, data, slots, rows, heads, q, "many rows")
+
+
+def test_cross_many_rows_of_every_size(gpu):
+    """The many-row kernel with scores that rise from block to block, a sink, tiny and huge values, and queries that
+    are 0, NaN or infinite."""
+    print("case cross many rows, sizes", flush=True)
+    hd, heads, kvh, n = 64, 64, 8, 400
+    k, v = rows_of(75, 300, kvh, hd)
+    k *= np.linspace(0.05, 6.0, 300).astype(np.float32)[:, None, None]  # each block's largest score far above the last's
+    k[10, 0] *= 1e4
+    v[:64] *= 6e-8
+    v[200:210] = 65504.0
+    c = hip.CrossStates(1, kvh, hd, 1, 300)
+    c.set(0, [0], [300], k, v)
+    q = queries(76, n, heads, hd)
+    q[5], q[6] = 0.0, q[6] * 1e-25
+    q[7, 3, 1], q[8, 9, 0] = np.nan, -np.inf
+    got = c.attention(0, [0], [n], q, heads).reshape(n, heads, hd)
+    bad = np.zeros((n, heads), bool)
+    bad[7, 3] = bad[8, 9] = True
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    pick = np.array([0, 5, 6, 9, 100, 255, 399])
+    want, off = P.attention(q[pick], P.f16(k), P.f16(v), [300] * len(pick), 0.125)
+    near(got[pick], want, off, "sizes")
+    v[130, 2, 9] = np.nan
+    c.set(0, [0], [300], k, v)
+    again = c.attention(0, [0], [n], q, heads).reshape(n, heads, hd)
+    nan = np.isnan(again) & ~np.isnan(got)
+    assert nan[:, 16:24, 9][~bad[:, 16:24]].all() and nan.sum() == (~bad[:, 16:24]).sum()

@@ -20,6 +20,8 @@ constexpr int MOST_CHUNKS = 128;
 // keeps the low part of an f16 pair clear of subnormal f16.
 constexpr float FIXED = 8323072.0f;  // 127 * 65536
 constexpr float PAIR = 1024.0f, LOG_PAIR = 10.0f;
+// How far (in powers of two) scores may pass a softmax's reference: p * PAIR stays within f16.
+constexpr float SLACK = 5.0f;
 
 // The larger of a value and the one 32 (16) lanes away: a swap of two copies
 // leaves a lane its own value in one and the other's in the other.
@@ -58,7 +60,7 @@ __device__ __forceinline__ void digits4(uint32_t x0, uint32_t x1, uint32_t x2, u
 // 16 n + 4 (l / 16) + r.
 template <int HDP>
 struct Running {
-    float m = -INFINITY;  // the largest score so far, in powers of two (the same in a column's lanes)
+    float m = -INFINITY;  // the sums' reference, in powers of two: the largest score so far but for SLACK
     float l = 0.0f;       // this lane's part of the sum of 2^(score - m)
     v4f acc[HDP / 16];
 
@@ -101,17 +103,19 @@ __device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mas
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum += u[i];
-    const float mn = __builtin_fmaxf(run.m, mb);
-    const float before = mn == run.m ? 1.0f : __builtin_amdgcn_exp2f(run.m - mn);
-    const float now = any ? __builtin_amdgcn_exp2f(mb - mn) : 0.0f;
-    run.m = mn;
-    run.l = __builtin_fmaf(now, sum, run.l * before);
-    if (__any(before != 1.0f)) {
+    // The reference moves, and the sums with it, only when a score passes it by more than SLACK.
+    if (__any(mb > run.m + SLACK)) {
+        const float mn = __builtin_fmaxf(run.m, mb);
+        const float before = mn == run.m ? 1.0f : __builtin_amdgcn_exp2f(run.m - mn);
+        run.m = mn;
+        run.l *= before;
 #pragma unroll
         for (int n = 0; n < HDP / 16; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) run.acc[n][r] *= before;
     }
+    const float now = any ? __builtin_amdgcn_exp2f(mb - run.m) : 0.0f;
+    run.l = __builtin_fmaf(now, sum, run.l);
     return now;
 }
 
@@ -420,7 +424,9 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
     const AttendSeq seq = a.s[si - 1];
     const int item = (int)blockIdx.y - seq.start;
-    const int tile = seq.chunks == 1 ? item : item / seq.chunks, chunk = item - tile * seq.chunks;
+    const int upto = seq.chunks == 1 ? item : item / seq.chunks, chunk = item - upto * seq.chunks;
+    // The last rows' tiles first: they see the most.
+    const int tile = (seq.rows * a.group - 1) / 16 - upto;
     const int columns = seq.rows * a.group, cols = min(columns - tile * 16, 16);
     // Column c's row and head: row0 + (rest + c) / group. The quotient is of small whole numbers, exact in f32.
     const int row0 = tile * 16 / a.group, rest = tile * 16 - row0 * a.group;
@@ -595,7 +601,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     // Every store of the workgroup is in memory before its arrival is counted.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    int* counter = a.counters + (seq.group + tile) * a.kv_heads + g;
+    int* counter = a.counters + (seq.group + upto) * a.kv_heads + g;
     if (t == 0) {
         const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         arrived = before + 1 == seq.chunks;
@@ -604,7 +610,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     __syncthreads();
     if (!arrived) return;
     // The chunks' largest scores and sums, then their outputs: a thread two dims of a column, its loads all in flight.
-    const size_t first = (size_t)(seq.part + tile * seq.chunks) * a.kv_heads + g;
+    const size_t first = (size_t)(seq.part + upto * seq.chunks) * a.kv_heads + g;
     float* tops = &part[0][0][0];
     float* sums = tops + 16 * MOST_CHUNKS;
     static_assert(sizeof(part) >= 2 * 16 * MOST_CHUNKS * sizeof(float), "a chunk's entries fit the waves' parts");
@@ -652,33 +658,24 @@ __device__ __forceinline__ void split2(float a, float b, float minus_one, uint32
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// Four int8 codes as f16, exactly: the byte c + 128 below an exponent of 2^10 is 1152 + c.
-__device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& h01, uint32_t& h23) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const uint32_t u = c ^ 0x80808080u;
-    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
-    const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
-    h01 = __builtin_bit_cast(uint32_t, a);
-    h23 = __builtin_bit_cast(uint32_t, b);
-}
-
-// Attention where a sequence has many query columns: workgroup (g, item) takes
-// 64 columns of a sequence (column r * group + c: row r, head g * group + c),
-// a wave 16 of them over every key block they see. The blocks pass through
-// shared memory as f16 fragments, once for the four waves, the next one's
-// loads in flight while one is worked on; int8 codes are widened on the way
-// (exactly), so both products run on f16 pairs of the queries and
-// probabilities. Against the integer form above, whose three digits need
-// 420 vector instructions a block and 16 columns, this takes 230, and those
-// are what binds; the columns of later rows start first (they see the most).
-// A probability is a pair relative to the running maximum, times PAIR: what
-// is lost of it is below 2^-34 of the largest.
-template <int HDP, bool PAGED>
-__global__ __launch_bounds__(256, HDP == 128 ? 2 : PAGED ? 3 : 4) void attend_rows_kernel(AttendArgs a) {
+// Attention to states where a slot is asked by many query columns: workgroup
+// (g, item) takes 64 columns of a slot (column r * group + c: row r, head
+// g * group + c), a wave 16 of them over every key block. The blocks pass
+// through shared memory, once for the four waves, the next one's loads in
+// flight while one is worked on. What binds is the issue of vector and matrix
+// instructions together: about 150 and 32 a block and wave (64 wide), the sum
+// of their cycles near the time the compute units are busy. (32 columns a
+// wave read each fragment once for two tiles, but leave half the waves: 63 us
+// for 448 rows over each of 8 audios where this takes 55.)
+//
+// A probability is an f16 pair relative to a reference within SLACK of the
+// running maximum, times PAIR; what a pair loses is below 2^-34 of the
+// largest, so sums run on across blocks.
+template <int HDP>
+__global__ __launch_bounds__(256, HDP == 64 ? 4 : 2) void attend_rows_kernel(AttendArgs a) {
     constexpr int NT = HDP / 16, KS = HDP / 32, F = BLOCK_TOKENS * HDP * 2 / 8 / 256;  // 16-byte pieces a thread
     constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
-    __shared__ __align__(16) _Float16 kv[2][BLOCK];
+    __shared__ __align__(16) _Float16 kv[BLOCK];
     const int t = threadIdx.x, lane = t % WAVE, col = lane % 16, lq = lane / 16;
     const int w = __builtin_amdgcn_readfirstlane(t / WAVE);
     const int g = blockIdx.x;
@@ -688,91 +685,26 @@ __global__ __launch_bounds__(256, HDP == 128 ? 2 : PAGED ? 3 : 4) void attend_ro
         for (int i = 0; i < CALL_SEQS; i += WAVE) si += __popcll(__ballot(a.s[i + lane].start <= (int)blockIdx.y));
     const AttendSeq seq = a.s[si - 1];
     const int columns = seq.rows * a.group;
-    const int wide = (columns + 63) / 64 - 1 - ((int)blockIdx.y - seq.start);  // 64 columns, the last ones first
-    const int tile = wide * 4 + w, cols = min(columns - tile * 16, 16);  // may be 0 or less: a wave without columns
-    const int row0 = tile * 16 / a.group, rest = tile * 16 - row0 * a.group;
-    const int r = (int)(((float)(rest + col) + 0.5f) * (1.0f / (float)a.group)), h = g * a.group + rest + col - r * a.group;
-    const bool valid = col < cols;
-    // Keys: what the lane's column sees, the least of the wave's columns, the most of the workgroup's.
-    const int ahead = PAGED ? seq.len - seq.rows + 1 : seq.len;
-    const int seen = valid ? ahead + (PAGED ? row0 + r : 0) : 0;
-    const int least = PAGED ? ahead + row0 : ahead;
-    const int most = PAGED ? ahead + (min(wide * 64 + 63, columns - 1)) / a.group : ahead;
-    const int end = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
-    const int full = PAGED ? seq.len / BLOCK_TOKENS : 0;
+    const int tile = ((int)blockIdx.y - seq.start) * 4 + w;  // the wave's
+    const bool idle = tile * 16 >= columns;  // a wave without columns: it moves blocks only
+    const int end = (seq.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+    const _Float16* states = a.f16 + ((size_t)seq.place * a.kv_heads + g) * a.blocks * BLOCK;
 
-    // The thread's pieces of the next block: codes (4 * F values in F / 2 pieces) or halves.
-    uint4 piece[F];
-    float2 sc = make_float2(1.0f, 1.0f), sn = sc;
-    const int* table = PAGED ? a.table + (size_t)seq.place * a.table_stride : nullptr;
+    uint4 piece[F];  // the thread's pieces of the next block
     auto fetch = [&](int b) {
-        if (PAGED && b < full) {
-            const size_t at = (size_t)table[b] * a.kv_heads + g;
-            const uint8_t* src = a.codes + at * BLOCK;
-            sn = a.scales[at];
 #pragma unroll
-            for (int i = 0; i < F / 2; ++i) piece[i] = gload_u4(src + i * 4096 + t * 16);
-        } else {
-            const _Float16* src = PAGED ? a.f16 + ((size_t)seq.place * a.kv_heads + g) * BLOCK
-                                        : a.f16 + (((size_t)seq.place * a.kv_heads + g) * a.blocks + b) * BLOCK;
-            sn = make_float2(1.0f, 1.0f);
-#pragma unroll
-            for (int i = 0; i < F; ++i) piece[i] = gload_u4(src + i * 2048 + t * 8);
-        }
+        for (int i = 0; i < F; ++i) piece[i] = gload_u4(states + b * BLOCK + i * 2048 + t * 8);
     };
-    // Into shared memory as f16 fragments; of an open block, values behind the last token as 0. Returns whether an
-    // open block holds a NaN value.
-    auto put_block = [&](int b, _Float16* to) {
-        bool nan = false;
-        if (PAGED && b < full) {
-#pragma unroll
-            for (int i = 0; i < F / 2; ++i) {
-                const uint32_t c[4] = {piece[i].x, piece[i].y, piece[i].z, piece[i].w};
-                uint32_t x[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) codes_to_f16(c[j], x[2 * j], x[2 * j + 1]);
-                // Piece u = 256 i + t of the block: fragment f, its lane l. K: 16 dims of a token, two lanes' worth
-                // of one f16 fragment. V: 16 tokens of a dim, one lane's in each of two fragments.
-                const int f = i * 4 + t / WAVE, l = lane;
-                int at0, at1;
-                if (i < F / 4) {
-                    const int tile16 = f / (HDP / 64), ks = f % (HDP / 64) * 2 + l / 32;
-                    at0 = ((tile16 * KS + ks) * 64 + l / 16 % 2 * 32 + l % 16) * 8;
-                    at1 = at0 + 16 * 8;
-                } else {
-                    at0 = BLOCK / 2 + ((f - NT) * 2 * 64 + l) * 8;
-                    at1 = at0 + 64 * 8;
-                }
-                *(uint4*)(to + at0) = make_uint4(x[0], x[1], x[2], x[3]);
-                *(uint4*)(to + at1) = make_uint4(x[4], x[5], x[6], x[7]);
-            }
-            return nan;
-        }
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            uint4 x = piece[i];
-            if (PAGED && i >= F / 2) {
-                const int s = (i * 4 + t / WAVE) % 2, tokens = seq.len - b * BLOCK_TOKENS;
-                uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int tok = 32 * s + 16 * (j / 2) + 4 * lq + 2 * (j % 2);
-                    y[j] &= tok + 1 < tokens ? 0xffffffffu : tok < tokens ? 0xffffu : 0u;
-                    nan |= (((y[j] & 0x7fff7fffu) + 0x03ff03ffu) & 0x80008000u) != 0;
-                }
-                x = make_uint4(y[0], y[1], y[2], y[3]);
-            }
-            *(uint4*)(to + i * 2048 + t * 8) = x;
-        }
-        return nan;
-    };
-
-    fetch(0);
-    // The lane's query values: dims 32 ks + 8 lq + i of its column, as f16 pairs.
+    if (end > 0) fetch(0);
+    // The lane's column: row and head.
+    const int row0 = tile * 16 / a.group, x0 = tile * 16 - row0 * a.group + col;
+    const int r = (int)(((float)x0 + 0.5f) * (1.0f / (float)a.group)), row = row0 + r, head = g * a.group + x0 - r * a.group;
+    const bool valid = tile * 16 + col < columns;
+    // Its query values: dims 32 ks + 8 lq + i, as f16 pairs.
     v8h qh[KS], ql[KS];
     float step;
     {
-        const float* q = valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q;
+        const float* q = valid ? a.q + (size_t)(seq.first + row) * a.qs + (size_t)head * a.hd : a.q;
         float v[KS][8], top = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -815,145 +747,90 @@ __global__ __launch_bounds__(256, HDP == 128 ? 2 : PAGED ? 3 : 4) void attend_ro
     }
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // m: the reference of the sums
     v4f acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-    bool nan = end > 0 && put_block(0, kv[0]);
-    int any_nan_here = __syncthreads_or(PAGED && nan);
     for (int b = 0; b < end; ++b) {
-        const _Float16* k = kv[b % 2];
-        sc = sn;
+#pragma unroll
+        for (int i = 0; i < F; ++i) *(uint4*)(kv + i * 2048 + t * 8) = piece[i];
+        __syncthreads();
         if (b + 1 < end) fetch(b + 1);
-        if (cols > 0 && (!PAGED || b * BLOCK_TOKENS < ahead + row0 + (rest + cols - 1) / a.group)) {
-            float u[16];
+        if (!idle) {
+            const _Float16* k = kv + lane * 8;
+            v4f u[4];
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 4; ++i) u[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const v8h kf = *(const v8h*)(k + (tt * KS + ks) * 512 + lane * 8);
-                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[ks], c, 0, 0, 0);
-                    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[ks], c, 0, 0, 0);
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v8h kf = *(const v8h*)(k + (i * KS + ks) * 512);
+                    u[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[ks], u[i], 0, 0, 0);
+                    u[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[ks], u[i], 0, 0, 0);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) u[4 * tt + i] = c[i];
-            }
-            const float f = step * sc.x;
-            const int sees = seen - b * BLOCK_TOKENS;
-            const bool mask = (b + 1) * BLOCK_TOKENS > least;
+            const int tokens = seq.len - b * BLOCK_TOKENS;
+            const bool mask = tokens < BLOCK_TOKENS;
+            v8h ph[2], pl[2];
             if (mask) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (16 * (i / 4) + 4 * lq + i % 4 >= sees) u[i] = -INFINITY;
+                    if (16 * (i / 4) + 4 * lq + i % 4 >= tokens) u[i / 4][i % 4] = -INFINITY;
             }
-            float top = u[0];
+            float top = u[0][0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i]);
-            top = column_max(top);
-            // (A column that sees nothing of the block: -inf, also where its scale is 0 or NaN.)
-            const float mn = __builtin_fmaxf(m, top > -INFINITY ? top * f : -INFINITY);
-            const float before = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            const float ref = mn > -INFINITY ? mn - LOG_PAIR : 0.0f;
-            m = mn;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(u[i], f, -ref));
-            if (mask) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (16 * (i / 4) + 4 * lq + i % 4 >= sees) u[i] = 0.0f;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += u[i];
-            l = __builtin_fmaf(l, before, sum);
-            if (__any(before != 1.0f)) {
+            for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i / 4][i % 4]);
+            top = column_max(top) * step;
+            if (__any(top > m + SLACK)) {
+                const float mn = __builtin_fmaxf(m, top);
+                const float before = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= before;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[n][i] *= before;
             }
-            v8h ph[2], pl[2];
+            const float ref = (m > -INFINITY ? m : 0.0f) - LOG_PAIR;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(u[i / 4][i % 4], step, -ref));
+                u[i / 4][i % 4] = p;
+                sum += p;
+            }
+            l += sum;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 v4i hi, lo;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t x, y;
-                    split2(u[8 * s + 2 * i], u[8 * s + 2 * i + 1], minus_one, x, y);
+                    split2(u[2 * s + i / 2][2 * i % 4], u[2 * s + i / 2][2 * i % 4 + 1], minus_one, x, y);
                     hi[i] = (int)x;
                     lo[i] = (int)y;
                 }
                 ph[s] = __builtin_bit_cast(v8h, hi);
                 pl[s] = __builtin_bit_cast(v8h, lo);
             }
-            const _Float16* v = k + BLOCK / 2 + lane * 8;
-            if (PAGED && b < full) {
-                const float sv = sees > 0 ? sc.y : 0.0f;
+            const _Float16* v = kv + BLOCK / 2 + lane * 8;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    v4f c = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const v8h vf = *(const v8h*)(v + (2 * n + s) * 512);
-                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], c, 0, 0, 0);
-                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], c, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][i] = __builtin_fmaf(c[i], sv, acc[n][i]);
+                for (int s = 0; s < 2; ++s) {
+                    const v8h vf = *(const v8h*)(v + (2 * n + s) * 512);
+                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], acc[n], 0, 0, 0);
+                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], acc[n], 0, 0, 0);
                 }
-            } else {
-                // As open_values: a NaN value counts for the columns that see its token and no others.
-                if (PAGED && any_nan_here) {
-                    v8h sees16[2];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        sees16[i / 8][i % 8] = (_Float16)(16 * (i / 4) + 4 * lq + i % 4 < sees ? 1.0f : 0.0f);
-                    for (int n = 0; n < NT; ++n) {
-                        v4f count = v4f{0.0f, 0.0f, 0.0f, 0.0f}, c = count;
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            v8h vf = *(const v8h*)(v + (2 * n + s) * 512), is;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const _Float16 x = vf[i];
-                                is[i] = (_Float16)(x != x ? 1.0f : 0.0f);
-                                vf[i] = x != x ? (_Float16)0.0f : x;
-                            }
-                            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees16[s], count, 0, 0, 0);
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], c, 0, 0, 0);
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], c, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int nn = 0; nn < NT; ++nn)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (nn == n) acc[nn][i] += count[i] > 0.0f ? NAN : c[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            const v8h vf = *(const v8h*)(v + (2 * n + s) * 512);
-                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[s], acc[n], 0, 0, 0);
-                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[s], acc[n], 0, 0, 0);
-                        }
-                }
-            }
         }
-        // The next block goes where the block before this one was: every wave has passed the last barrier.
-        nan = b + 1 < end && put_block(b + 1, kv[(b + 1) % 2]);
-        if (PAGED && b + 1 == full)
-            any_nan_here = __syncthreads_or(nan);
-        else
-            __syncthreads();
+        __syncthreads();  // the block is read
     }
     l = column_sum(l);
     if (!valid) return;
+    // No key at all: 0.
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float* out = a.out + ((size_t)(seq.first + row0 + r) * a.kv_heads * a.group + h) * a.hd;
+    float* out = a.out + ((size_t)(seq.first + row) * a.kv_heads * a.group + head) * a.hd;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -971,8 +848,14 @@ constexpr long long MOST_TILES = 50000;
 constexpr long long SPLIT_ITEMS = 1024;
 // Workgroups of 8 waves that the compute units take at once.
 constexpr long long FEW_ITEMS = 256;
-// Columns of a key head from which the many-row kernel takes a sequence.
-constexpr long long MANY_COLUMNS = 64;
+// Columns of a key head from which the many-row kernel takes a slot, and the
+// least workgroups it takes: with fewer its serial pass over the blocks is the
+// longer one. 64 wide, 20 heads, us here and on attend_kernel: 320 workgroups
+// 47 and 37, 500 57 and 68, 2000 120 and 165; 128 wide: 256 54 and 53, 392 92
+// and 102, 1568 186 and 235. (The same form for a paged cache, codes widened
+// into shared memory, was no shorter than attend_kernel: 1564 rows after 1000
+// tokens 102 and 71.)
+constexpr long long MANY_COLUMNS = 64, MANY_ITEMS = 384;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
     memory.alloc(SPLIT_ITEMS * (16 * ((size_t)hdp * 4 + 8) + 4));
@@ -990,12 +873,23 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     const auto tiles = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 15) / 16; };
     const auto blocks = [](const AttendSeq& q) { return (q.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS; };
     a.aligned = a.hd % 4 == 0 && a.qs % 4 == 0 && (uintptr_t)a.q % 16 == 0;
-    // Sequences of many columns in launches of their own.
+    // Slots that many columns ask, in launches of their own.
     std::vector<AttendSeq> few, many;
-    for (const AttendSeq& q : seqs)
-        if (q.rows) ((long long)q.rows * a.group >= MANY_COLUMNS ? many : few).push_back(q);
+    const auto wide = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 63) / 64; };
+    long long wides = 0;
+    for (const AttendSeq& q : seqs) {
+        if (!q.rows) continue;
+        const bool is = !paged && (long long)q.rows * a.group >= MANY_COLUMNS;
+        if (is) wides += wide(q);
+        (is ? many : few).push_back(q);
+    }
+    if (wides * a.kv_heads < MANY_ITEMS) {
+        few.insert(few.end(), many.begin(), many.end());
+        many.clear();
+    }
+    // The longest first, so that the last workgroups are short.
+    std::stable_sort(many.begin(), many.end(), [](const AttendSeq& x, const AttendSeq& y) { return x.len > y.len; });
     for (size_t at = 0; at < many.size();) {
-        const auto wide = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 63) / 64; };
         long long items = 0;
         for (a.n = 0; at < many.size() && a.n < CALL_SEQS; ++at) {
             AttendSeq q = many[at];
@@ -1006,8 +900,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
             a.s[a.n++] = q;
         }
         for (int i = a.n; i < CALL_SEQS; ++i) a.s[i].start = INT_MAX;
-        auto kernel = hdp == 64 ? (paged ? attend_rows_kernel<64, true> : attend_rows_kernel<64, false>)
-                                : (paged ? attend_rows_kernel<128, true> : attend_rows_kernel<128, false>);
+        auto kernel = hdp == 64 ? attend_rows_kernel<64> : attend_rows_kernel<128>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)a.kv_heads, (unsigned)items), dim3(256), 0, s, a);
         TRIT_HIP(hipGetLastError());
     }
@@ -1017,6 +910,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
         int most = 0;
         size_t to = from;
         for (a.n = 0; to < few.size() && a.n < CALL_SEQS; ++to) {
+            if (tiles(few[to]) > MOST_TILES) fail("attention: more query rows than one launch takes");
             if (a.n && whole + tiles(few[to]) > MOST_TILES) break;
             whole += tiles(few[to]);
             work += tiles(few[to]) * blocks(few[to]);
