@@ -4,6 +4,7 @@
 #include <climits>
 
 #include "attend.h"
+#include "blocks.h"
 #include "device.h"
 
 namespace trit {
@@ -23,18 +24,6 @@ constexpr float PAIR = 1024.0f, LOG_PAIR = 10.0f;
 // How far (in powers of two) scores may pass a softmax's reference: p * PAIR stays within f16.
 constexpr float SLACK = 5.0f;
 
-// The larger of a value and the one 32 (16) lanes away: a swap of two copies
-// leaves a lane its own value in one and the other's in the other.
-__device__ __forceinline__ float other_half_max(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float other_row_max(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
 // The largest over a column's four lanes (l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float column_max(float v) { return other_half_max(other_row_max(v)); }
 __device__ __forceinline__ float column_sum(float v) {

@@ -26,37 +26,43 @@ struct SetArgs {
 // Workgroup (x, g, 2 i + which): block x of keys (which 0) or values (1) of
 // head g of the i-th slot, zero past its keys and past head_dim. (Values of
 // keys that are not there meet probabilities of 0.)
+template <int HDP, bool V>
+__device__ __forceinline__ void set_block(_Float16* to, int hd, int keys, const float* rows, long long stride,
+                                          bool aligned, _Float16* out) {
+    constexpr int G = BlockShare<HDP>::GROUPS;
+    const int t = threadIdx.x, first = blockIdx.x * BLOCK_TOKENS;
+    float h[4 * G];
+    load_share<HDP, V>(rows, stride, first, keys, hd, aligned, h);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+        int tok, e;
+        share_at<HDP, V>(i, tok, e);
+        _Float16 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool valid = first + tok + (V ? j : 0) < keys && e + (V ? 0 : j) < hd;
+            x[j] = valid ? held(h[4 * i + j]) : (_Float16)0.0f;
+        }
+        __builtin_memcpy(out + half_at<HDP, V>(tok, e), x, 8);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BLOCK_TOKENS * HDP / 8; i += THREADS) *(uint4*)(to + (i + t) * 8) = *(const uint4*)(out + (i + t) * 8);
+}
 template <int HDP>
 __global__ __launch_bounds__(THREADS) void set_kernel(_Float16* states, int blocks, int kv_heads, int hd, SetArgs a,
                                                       const float* k, long long ks, const float* v, long long vs,
                                                       bool aligned) {
-    constexpr int G = BlockShare<HDP>::GROUPS;
     __shared__ __align__(16) _Float16 out[BLOCK_TOKENS * HDP];
-    const bool which = blockIdx.z % 2;
-    const int g = blockIdx.y, t = threadIdx.x, first = blockIdx.x * BLOCK_TOKENS;
+    const int g = blockIdx.y;
     const SetSeq s = a.s[blockIdx.z / 2];
-    if (first >= s.keys) return;
-    const long long stride = which ? vs : ks;
-    float h[4 * G];
-    load_share<HDP>(which, (which ? v : k) + (size_t)s.first * stride + (size_t)g * hd, stride, first, s.keys, hd,
-                    aligned, h);
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-        int tok, e;
-        share_at<HDP>(which, i, tok, e);
-        _Float16 x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool valid = first + tok + (which ? j : 0) < s.keys && e + (which ? 0 : j) < hd;
-            x[j] = valid ? held(h[4 * i + j]) : (_Float16)0.0f;
-        }
-        __builtin_memcpy(out + half_at<HDP>(which, tok, e), x, 8);
-    }
-    __syncthreads();
-    uint4* dst =
-        (uint4*)(states + ((((size_t)s.slot * kv_heads + g) * blocks + blockIdx.x) * 2 + which) * (BLOCK_TOKENS * HDP));
-#pragma unroll
-    for (int i = 0; i < BLOCK_TOKENS * HDP / 8; i += THREADS) dst[i + t] = *(const uint4*)(out + (i + t) * 8);
+    if ((int)blockIdx.x * BLOCK_TOKENS >= s.keys) return;
+    _Float16* to =
+        states + (((size_t)s.slot * kv_heads + g) * blocks + blockIdx.x) * 2 * (BLOCK_TOKENS * HDP);
+    if (blockIdx.z % 2)
+        set_block<HDP, true>(to + BLOCK_TOKENS * HDP, hd, s.keys, v + (size_t)s.first * vs + (size_t)g * hd, vs, aligned, out);
+    else
+        set_block<HDP, false>(to, hd, s.keys, k + (size_t)s.first * ks + (size_t)g * hd, ks, aligned, out);
 }
 
 }  // namespace
