@@ -516,9 +516,11 @@ int trit_hip_paged_read_device(TritHipPagedCache *cache, int layer, const int32_
  * sequence after another, heads * head_dim f32 each (_device: stride q_stride
  * floats); out is dense, as q's rows. Query head h reads key head h / (heads /
  * kv_heads). scale: on the scores, 0 for 1/sqrt(head_dim). Sums and softmax
- * in f32, the queries and probabilities to 24 bits; a NaN in the cache
- * reaches the rows that see its token (its block's, when that is full).
- * rows[i] may be 1 (a decode step) up to the tokens held (a prompt). */
+ * in f32, the queries and probabilities to 24 bits (22 where a block holds
+ * f16); a score that f32 does not hold gives NaN. A NaN in the cache reaches
+ * the rows that see its token (its block's, when that is full), one in a
+ * query its own row and head. rows[i] may be 0, 1 (a decode step), up to the
+ * tokens held (a prompt); rows[i] * heads / kv_heads at most 800000. */
 int trit_hip_paged_attention(TritHipPagedCache *cache, int layer, const int32_t *sequences, const int32_t *rows, int n,
                              const float *q, int heads, float scale, float *out);
 int trit_hip_paged_attention_device(TritHipPagedCache *cache, int layer, const int32_t *sequences,
@@ -549,7 +551,7 @@ int trit_hip_cross_set_device(TritHipCross *cross, int layer, const int32_t *slo
 int trit_hip_cross_keys(TritHipCross *cross, int layer, int slot);
 
 /* Attention of rows[i] query rows to every key of slots[i] (a slot may be
- * named more than once), q, out, heads and scale as
+ * named more than once), q, out, heads, scale and precision as
  * trit_hip_paged_attention. Rows of a slot of no keys are 0. */
 int trit_hip_cross_attention(TritHipCross *cross, int layer, const int32_t *slots, const int32_t *rows, int n,
                              const float *q, int heads, float scale, float *out);

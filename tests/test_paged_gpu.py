@@ -469,3 +469,89 @@ def test_capture_is_refused(gpu):
     g.replay()
     torch.cuda.synchronize()
     assert (out == 1.0).all()
+
+
+def test_a_failed_resize_leaves_the_cache_as_it_was(gpu):
+    """More memory than the card has: refused, and the next calls know nothing of it."""
+    print("case resize beyond the card", flush=True)
+    c, ids, data = filled(128, 8, [70, 3], layers=4)
+    before = c.info()
+    with pytest.raises(hip.TritError, match="memory"):
+        c.resize(1 << 24)  # 8 TB
+    assert c.info() == before
+    new = rows_of(41, 2, 8, 128)
+    for layer in range(4):
+        c.append(layer, ids, [1, 1], *new)
+    held = [(np.concatenate([k, new[0][i:i + 1]]), np.concatenate([v, new[1][i:i + 1]])) for i, (k, v) in enumerate(data)]
+    check_attention(c, ids, held, [1, 2], 16, layer=3, what="after")
+
+
+def test_two_threads(gpu):
+    """Calls of two threads, each on its own stream, take turns."""
+    print("case two threads", flush=True)
+    import threading
+
+    c, ids, data = filled(64, 2, [700, 90], pages=60, sequences=8)
+    q = queries(5, 2, 4, 64)
+    want = c.attention(0, ids, [1, 1], q, 4)
+    bad = []
+
+    def work(mine):
+        try:
+            hip.init(0)
+            for step in range(20):
+                if not same(c.attention(0, ids, [1, 1], q, 4), want):
+                    bad.append("attention")
+                child = c.fork([ids[mine]])
+                k, v = rows_of(100 * mine + step, 70, 2, 64)
+                c.append(0, child, [70], k, v)
+                n = len(data[mine][0])
+                got = c.read(0, child, [n], [70])
+                held = P.held(np.concatenate([data[mine][0], k]))[n:]
+                if not same(got[0], flat(held)):
+                    bad.append("append")
+                c.close(child)
+        except Exception as e:  # noqa: BLE001
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:3]
+
+
+def test_a_step_of_a_batch(gpu):
+    """A decoder layer's step as it is used: beams forked, a token appended, self attention, cross attention to their
+    audio's states, the beams chosen again."""
+    print("case a batch's steps", flush=True)
+    hd, kvh, heads, audios, beams = 64, 4, 4, 3, 4
+    states = [rows_of(200 + a, n, kvh, hd) for a, n in enumerate((150, 64, 31))]
+    cross = hip.CrossStates(2, kvh, hd, audios, 150)
+    cache = hip.PagedCache(2, kvh, hd, 60, audios * beams)
+    prompt = [rows_of(210 + a, n, kvh, hd) for a, n in enumerate((60, 3, 127))]
+    first = cache.open(audios)
+    for layer in range(2):
+        cross.set(layer, range(audios), [len(k) for k, _ in states], *(np.concatenate(x) for x in zip(*states)))
+        cache.append(layer, first, [len(k) for k, _ in prompt], *(np.concatenate(x) for x in zip(*prompt)))
+    ids = np.concatenate([np.concatenate([first[a:a + 1], cache.fork([first[a]] * (beams - 1))]) for a in range(audios)])
+    held = [prompt[a] for a in range(audios) for _ in range(beams)]
+    r = np.random.default_rng(8)
+    n = audios * beams
+    for step in range(8):
+        new = rows_of(300 + step, n, kvh, hd)
+        q = queries(400 + step, n, heads, hd)
+        held = [(np.concatenate([k, new[0][i:i + 1]]), np.concatenate([v, new[1][i:i + 1]]))
+                for i, (k, v) in enumerate(held)]
+        for layer in range(2):
+            cache.append(layer, ids, [1] * n, *new)
+            check_attention(cache, ids, held, [1] * n, heads, layer=layer, q=q, what=f"step {step}")
+            got = cross.attention(layer, range(audios), [beams] * audios, q, heads).reshape(n, heads, hd)
+            for a, (k, v) in enumerate(states):
+                rows = slice(a * beams, (a + 1) * beams)
+                want, off = P.attention(q[rows], P.f16(k), P.f16(v), [len(k)] * beams, 0.125)
+                near(got[rows], want, off, f"cross {step}")
+        parents = np.concatenate([a * beams + r.integers(0, beams, beams) for a in range(audios)])
+        cache.reorder(ids, ids[parents])
+        held = [held[p] for p in parents]

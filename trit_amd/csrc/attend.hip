@@ -587,7 +587,9 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         put(a.sums + at * HDP + e, o);
         if (e == 0) put(a.tops + at, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(m));
     }
-    // Every store of the workgroup is in memory before its arrival is counted.
+    // Every store of the workgroup is in memory before its arrival is counted: put() writes through the L2, so the
+    // wait is enough. (A release fence also writes back whatever else the L2 holds: the 32 ragged requests 39.8 us,
+    // without 32.2.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     int* counter = a.counters + (seq.group + upto) * a.kv_heads + g;

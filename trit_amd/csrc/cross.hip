@@ -90,6 +90,8 @@ struct TritHipCross {
             fail("cross attention: the states live on device " + std::to_string(device) +
                  ", the calling thread uses device " + std::to_string(now != device ? now : device_id()));
         hipStream_t s = stream_ ? (hipStream_t)stream_ : stream();
+        // An error that an earlier call returned (a failed allocation) is not this call's.
+        (void)hipGetLastError();
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
         TRIT_HIP(hipStreamIsCapturing(s, &status));
         if (status != hipStreamCaptureStatusNone)

@@ -10,6 +10,8 @@
 #include <queue>
 #include <stdexcept>
 #include <string>
+#include <unordered_map>
+#include <utility>
 #include <vector>
 
 namespace trit {
@@ -126,29 +128,27 @@ class PageBook {
               std::vector<PageMove>& pages, std::vector<Entry>& entries) {
         for (int i = 0; i < n; ++i) even(ids[i]);
         into.need_ids(n);
-        std::vector<int> to((size_t)this->pages(), -1), fresh;
+        // The copy of each page, and whether a sequence holds it yet (take_page counts the first).
+        std::unordered_map<int, std::pair<int, bool>> to;
+        std::vector<int> fresh;
         for (int i = 0; i < n; ++i)
             for (int p : seqs_[(size_t)ids[i]].pages)
-                if (to[(size_t)p] < 0) {
-                    to[(size_t)p] = 0;
-                    fresh.push_back(p);
-                }
+                if (to.emplace(p, std::make_pair(-1, false)).second) fresh.push_back(p);
         into.need_pages((long long)fresh.size());
         const std::vector<int> from(ids, ids + n);
         for (int p : fresh) {
-            to[(size_t)p] = into.take_page();
-            pages.push_back({p, to[(size_t)p]});
+            to[p].first = into.take_page();
+            pages.push_back({p, to[p].first});
         }
-        std::vector<int> held((size_t)into.pages(), 0);
         for (int i = 0; i < n; ++i) {
             const int id = into.take_id();
             Seq& d = into.seqs_[(size_t)id];
             const Seq& s = seqs_[(size_t)from[(size_t)i]];
             d.len = s.len;
             for (size_t b = 0; b < s.pages.size(); ++b) {
-                const int p = to[(size_t)s.pages[b]];
-                // take_page counted the first holder.
-                if (held[(size_t)p]++) ++into.refs_[(size_t)p];
+                auto& [p, held] = to[s.pages[b]];
+                if (held) ++into.refs_[(size_t)p];
+                held = true;
                 d.pages.push_back(p);
                 entries.push_back({d.row, (int)b, p});
             }
