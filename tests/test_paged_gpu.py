@@ -154,6 +154,17 @@ def test_attention(gpu, hd, heads, kvh, lens, rows):
     check_attention(c, ids, data, rows, heads, what="attention")
 
 
+# Rows enough that a workgroup takes two tiles of columns: odd numbers of tiles, sequences that ask nothing or little.
+@pytest.mark.parametrize("hd,heads,kvh,lens,rows", [
+    (20, 16, 8, [1300, 5, 1000, 900, 70], [1000, 0, 1000, 300, 1]),
+    (128, 24, 8, [701, 690], [701, 690]),
+])
+def test_attention_of_many_rows(gpu, hd, heads, kvh, lens, rows):
+    print(f"case attention of many rows {hd} {heads}/{kvh} lens {lens} rows {rows}", flush=True)
+    c, ids, data = filled(hd, kvh, lens)
+    check_attention(c, ids, data, rows, heads, what="attention of many rows")
+
+
 def test_scale_and_layers(gpu):
     print("case scale, layers", flush=True)
     c, ids, data = filled(64, 2, [70, 129], layers=3)

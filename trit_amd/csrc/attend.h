@@ -77,7 +77,7 @@ struct AttendArgs {
     uint64_t* tops = nullptr;
     int* counters = nullptr;
     int chunk = 0;
-    bool aligned = false;  // 16-byte loads of the queries
+    bool aligned = false, aligned_out = false;  // 16-byte loads of the queries, stores of the outputs
     int n = 0;
     AttendSeq s[CALL_SEQS];
 };

@@ -379,9 +379,6 @@ __global__ void clear_kernel(int* p, int n) {
 
 // Words that other workgroups of the launch read: to and from memory past the
 // caches that a reader on another XCD does not share.
-__device__ __forceinline__ void put(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 __device__ __forceinline__ void put(uint64_t* p, uint64_t v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -390,16 +387,17 @@ __device__ __forceinline__ float2 get(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// Block (item): sequence, key head g, a tile of 16 columns (query row r, head
-// g * group + c of it: column r * group + c) and a chunk of its key blocks.
-// The four waves take the chunk's blocks in turn and join their sums in shared
-// memory. Of the workgroups of a tile's chunks the last to end joins theirs,
-// in the chunks' order.
-template <int HDP, bool PAGED, int WAVES>
+// Block (item): sequence, key head g, TILES tiles of 16 columns (query row r,
+// head g * group + c of it: column r * group + c) and a chunk of its key blocks
+// (two tiles: all of them). Each tile's waves take the chunk's blocks in turn
+// and join their sums in shared memory. Of the workgroups of a tile's chunks
+// the last to end joins theirs, in the chunks' order.
+template <int HDP, bool PAGED, int WAVES, int TILES = 1>
 __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     constexpr int NT = HDP / 16, KS = HDP / 64, PS = HDP + 4;
+    constexpr int KEYED = WAVES / TILES;  // waves that share a tile's keys
     constexpr size_t BLOCK = 2 * BLOCK_TOKENS * HDP;
-    __shared__ Queries<HDP, PAGED> qs;
+    __shared__ Queries<HDP, PAGED> queries[TILES];
     __shared__ float top[WAVES][16], sum[WAVES][16];
     __shared__ __align__(16) float part[WAVES][16][PS];
     __shared__ bool arrived;
@@ -415,31 +413,45 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     const int item = (int)blockIdx.y - seq.start;
     const int upto = seq.chunks == 1 ? item : item / seq.chunks, chunk = item - upto * seq.chunks;
     // The last rows' tiles first: they see the most.
-    const int tile = (seq.rows * a.group - 1) / 16 - upto;
-    const int columns = seq.rows * a.group, cols = min(columns - tile * 16, 16);
+    const int columns = seq.rows * a.group;
+    const int tile = ((columns - 1) / (16 * TILES) - upto) * TILES, cols = min(columns - tile * 16, 16 * TILES);
+    // The wave's tile of the workgroup's, its columns (none: 0 or less) and its turn at the tile's keys.
+    const int mine = w / KEYED, turn = w % KEYED, own = min(cols - 16 * mine, 16);
+    const Queries<HDP, PAGED>& qs = queries[mine];
     // Column c's row and head: row0 + (rest + c) / group. The quotient is of small whole numbers, exact in f32.
     const int row0 = tile * 16 / a.group, rest = tile * 16 - row0 * a.group;
     const float per = 1.0f / (float)a.group;
     auto row_of = [&](int c) { return (int)(((float)(rest + c) + 0.5f) * per); };
 
     // The thread's query values are on their way while the first keys are.
-    float qv[NT];
+    float qv[TILES][NT];
     if (t < 256) {
-        const int c = t / 16, r = row_of(c), h = g * a.group + rest + c - r * a.group;
-        const bool valid = c < cols;
-        load_queries<HDP, PAGED>(valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q, valid,
-                                 a.aligned, a.hd, a.scale, qv);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            const int c = 16 * i + t / 16, r = row_of(c), h = g * a.group + rest + c - r * a.group;
+            const bool valid = c < cols;
+            load_queries<HDP, PAGED>(valid ? a.q + (size_t)(seq.first + row0 + r) * a.qs + (size_t)h * a.hd : a.q, valid,
+                                     a.aligned, a.hd, a.scale, qv[i]);
+        }
     }
-    // Keys the lane's column sees, and the tile's most and least.
+    auto put_all = [&] {
+        if (t < 256) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) put_queries<HDP, PAGED>(qv[i], queries[i]);
+        }
+        __syncthreads();
+    };
+    // Keys the lane's column sees, and the wave's tile's most and least.
     const int ahead = PAGED ? seq.len - seq.rows + 1 + row0 : seq.len;
-    const int most = PAGED ? ahead + (rest + cols - 1) / a.group : ahead;
-    const int seen = PAGED ? ahead + row_of(min(col, cols - 1)) : ahead;
+    const int least = PAGED ? ahead + (rest + 16 * mine) / a.group : ahead;
+    const int most = own <= 0 ? 0 : PAGED ? ahead + (rest + 16 * mine + own - 1) / a.group : ahead;
+    const int seen = PAGED ? ahead + row_of(16 * mine + min(col, max(own - 1, 0))) : ahead;
     const int b0 = chunk * a.chunk;
     const int all = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS, end = all < b0 + a.chunk ? all : b0 + a.chunk;
 
     Running<HDP> run;
     run.clear();
-    int b = b0 + w;
+    int b = b0 + turn;
     const uint32_t lane16 = lane * 16;
     if constexpr (PAGED) {
         const int full = seq.len / BLOCK_TOKENS;  // full blocks hold codes
@@ -457,32 +469,31 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             for (int i = 0; i < NT; ++i) kf[i] = load16(block + i * 1024, lane16);
 #pragma unroll
             for (int i = 0; i < NT; ++i) vf[i] = load16(block + BLOCK / 2 + i * 1024, lane16);
-            page = b + WAVES < last ? table[b + WAVES] : 0;
+            page = b + KEYED < last ? table[b + KEYED] : 0;
         }
-        if (t < 256) put_queries<HDP, PAGED>(qv, qs);
-        __syncthreads();
+        put_all();
         v4i qd[3][KS];
 #pragma unroll
         for (int j = 0; j < 3; ++j)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) qd[j][ks] = *(const v4i*)(qs.digits[j] + ks * 1024 + lane16);
         const float step = qs.top[col] * (LOG2E / FIXED);
-        for (; b < last; b += WAVES) {
+        for (; b < last; b += KEYED) {
             float u[16];
             codes_scores<HDP>(kf, qd, u);
-            const bool more = b + WAVES < last;
+            const bool more = b + KEYED < last;
             const float2 s0 = sc;
             const uint8_t* next = block;
             if (more) {
                 const size_t at = (size_t)page * a.kv_heads + g;
                 next = a.codes + at * BLOCK;
                 sc = a.scales[at];
-                page = b + 2 * WAVES < last ? table[b + 2 * WAVES] : 0;
+                page = b + 2 * KEYED < last ? table[b + 2 * KEYED] : 0;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024, lane16);
             }
             const float now =
-                block_softmax<HDP>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > ahead, seen - b * BLOCK_TOKENS, run);
+                block_softmax<HDP>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > least, seen - b * BLOCK_TOKENS, run);
             // A column that sees nothing of the block takes nothing of it, also where its scale is NaN.
             codes_values<HDP>(vf, u, now == 0.0f && seen <= b * BLOCK_TOKENS ? 0.0f : now * s0.y * (1.0f / FIXED), run);
             if (more) {
@@ -520,23 +531,22 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             load(kf, b, 0);
             if (AHEAD) load(vf, b, 1);
         }
-        if (t < 256) put_queries<HDP, PAGED>(qv, qs);
-        __syncthreads();
+        put_all();
         const float step = qs.top[col] * (LOG2E / PAIR);
-        for (; b < end; b += WAVES) {
+        for (; b < end; b += KEYED) {
             float u[16];
             f16_scores<HDP>(kf, qs.pairs[0], qs.pairs[1], u);
             if (!AHEAD) {
                 __builtin_amdgcn_sched_barrier(0);
                 load(vf, b, 1);
             }
-            const bool more = b + WAVES < end;
-            if (more && AHEAD) load(kf, b + WAVES, 0);
+            const bool more = b + KEYED < end;
+            if (more && AHEAD) load(kf, b + KEYED, 0);
             const float now =
                 block_softmax<HDP>(u, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
             f16_values<HDP>(vf, u, now, run);
-            if (more && !AHEAD) load(kf, b + WAVES, 0);
-            if (more && AHEAD) load(vf, b + WAVES, 1);
+            if (more && !AHEAD) load(kf, b + KEYED, 0);
+            if (more && AHEAD) load(vf, b + KEYED, 1);
         }
     }
     const float lsum = column_sum(run.l);
@@ -544,47 +554,62 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         top[w][col] = run.m;
         sum[w][col] = lsum;
     }
-    if (col < cols) {
+    if (col < own) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) *(v4f*)(part[w][col] + 16 * n + 4 * lq) = run.acc[n];
     }
     __syncthreads();
-    // The sums of the waves' parts, relative to their largest score m.
+    // Four dims of a column: the sums of the waves' parts, relative to their largest score m.
     auto joined = [&](int cc, int e, float& m, float& l) {
-        m = top[0][cc];
+        const int v0 = cc / 16 * KEYED, c = cc % 16;
+        m = top[v0][c];
 #pragma unroll
-        for (int v = 1; v < WAVES; ++v) m = __builtin_fmaxf(m, top[v][cc]);
-        float o = 0.0f;
+        for (int v = 1; v < KEYED; ++v) m = __builtin_fmaxf(m, top[v0 + v][c]);
+        v4f o = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         l = 0.0f;
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
+        for (int v = 0; v < KEYED; ++v) {
             // A wave that saw no key has sums of 0; NaN sums stay NaN.
-            const float f = top[v][cc] == m ? 1.0f : __builtin_amdgcn_exp2f(top[v][cc] - m);
-            o = __builtin_fmaf(part[v][cc][e], f, o);
-            l = __builtin_fmaf(sum[v][cc], f, l);
+            const float f = top[v0 + v][c] == m ? 1.0f : __builtin_amdgcn_exp2f(top[v0 + v][c] - m);
+            const v4f x = *(const v4f*)(part[v0 + v][c] + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], f, o[i]);
+            l = __builtin_fmaf(sum[v0 + v][c], f, l);
         }
         return o;
     };
-    auto store = [&](int cc, int e, float o, float l) {
+    auto store = [&](int cc, int e, v4f o, float l) {
         const int r = row_of(cc), h = g * a.group + rest + cc - r * a.group;
+        float* out = a.out + ((size_t)(seq.first + row0 + r) * a.kv_heads * a.group + h) * a.hd + e;
         // No key at all: 0.
-        if (e < a.hd)
-            a.out[((size_t)(seq.first + row0 + r) * a.kv_heads * a.group + h) * a.hd + e] = l == 0.0f ? 0.0f : o / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : o[i] * inv;
+        if (a.aligned_out) {
+            if (e < a.hd) *(v4f*)out = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e + i < a.hd) out[i] = o[i];
+        }
     };
-    if (seq.chunks == 1) {
-        for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
+    constexpr int QUADS = HDP / 4;
+    if (TILES == 2 || seq.chunks == 1) {
+        for (int i = t; i < cols * QUADS; i += WAVES * WAVE) {
             float m, l;
-            const float o = joined(i / HDP, i % HDP, m, l);
-            store(i / HDP, i % HDP, o, l);
+            const v4f o = joined(i / QUADS, i % QUADS * 4, m, l);
+            store(i / QUADS, i % QUADS * 4, o, l);
         }
         return;
     }
-    for (int i = t; i < cols * HDP; i += WAVES * WAVE) {
-        const int cc = i / HDP, e = i % HDP;
+    for (int i = t; i < cols * QUADS; i += WAVES * WAVE) {
+        const int cc = i / QUADS, e = i % QUADS * 4;
         float m, l;
-        const float o = joined(cc, e, m, l);
+        const v4f o = joined(cc, e, m, l);
         const size_t at = ((size_t)(seq.part + item) * a.kv_heads + g) * 16 + cc;
-        put(a.sums + at * HDP + e, o);
+        uint64_t* sums = (uint64_t*)(a.sums + at * HDP + e);
+        put(sums, (uint64_t)__float_as_uint(o[1]) << 32 | __float_as_uint(o[0]));
+        put(sums + 1, (uint64_t)__float_as_uint(o[3]) << 32 | __float_as_uint(o[2]));
         if (e == 0) put(a.tops + at, (uint64_t)__float_as_uint(l) << 32 | __float_as_uint(m));
     }
     // Every store of the workgroup is in memory before its arrival is counted: put() writes through the L2, so the
@@ -600,7 +625,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     }
     __syncthreads();
     if (!arrived) return;
-    // The chunks' largest scores and sums, then their outputs: a thread two dims of a column, its loads all in flight.
+    // The chunks' largest scores and sums, then their outputs: a thread four dims of a column, its loads all in flight.
     const size_t first = (size_t)(seq.part + upto * seq.chunks) * a.kv_heads + g;
     float* tops = &part[0][0][0];
     float* sums = tops + 16 * MOST_CHUNKS;
@@ -612,24 +637,25 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
         sums[i] = ml.y;
     }
     __syncthreads();
-    constexpr int PAIRS = HDP / 2;
-    for (int i = t; i < cols * PAIRS; i += WAVES * WAVE) {
-        const int cc = i / PAIRS, e = i % PAIRS * 2;
+    for (int i = t; i < cols * QUADS; i += WAVES * WAVE) {
+        const int cc = i / QUADS, e = i % QUADS * 4;
         const float* m = tops + cc * seq.chunks;
         float most = m[0];
         for (int v = 1; v < seq.chunks; ++v) most = __builtin_fmaxf(most, m[v]);
         float l = 0.0f;
-        float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 16
+        v4f o = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
         for (int v = 0; v < seq.chunks; ++v) {
-            const float2 x = get(a.sums + ((first + (size_t)v * a.kv_heads) * 16 + cc) * HDP + e);
+            const float* at = a.sums + ((first + (size_t)v * a.kv_heads) * 16 + cc) * HDP + e;
+            const float2 x = get(at), y = get(at + 2);
             const float f = m[v] == most ? 1.0f : __builtin_amdgcn_exp2f(m[v] - most);
             l = __builtin_fmaf(sums[cc * seq.chunks + v], f, l);
-            o.x = __builtin_fmaf(x.x, f, o.x);
-            o.y = __builtin_fmaf(x.y, f, o.y);
+            o[0] = __builtin_fmaf(x.x, f, o[0]);
+            o[1] = __builtin_fmaf(x.y, f, o[1]);
+            o[2] = __builtin_fmaf(y.x, f, o[2]);
+            o[3] = __builtin_fmaf(y.y, f, o[3]);
         }
-        store(cc, e, o.x, l);
-        store(cc, e + 1, o.y, l);
+        store(cc, e, o, l);
     }
 }
 
@@ -839,13 +865,22 @@ constexpr long long MOST_TILES = 50000;
 constexpr long long SPLIT_ITEMS = 1024;
 // Workgroups of 8 waves that the compute units take at once.
 constexpr long long FEW_ITEMS = 256;
+// The least workgroups of two tiles that a paged launch takes, where nine
+// tenths of the second ones are there (60 requests of a single tile 29 us with
+// one, 36 with room for two): a wave's keys are twice as many, so its fixed
+// part (queries, first loads, join) weighs half. 16/8 heads of 128, us with
+// one tile and with two: 3000 rows after 1000 tokens (1500 such workgroups)
+// 149 and 141, two prompts of 1564 (1568) 73 and 63, four (3136) 135 and 119;
+// 1564 rows after 1000 (784) 65.5 and 64.5, 1024 after 1024 (512) 38 and 39.
+// 20 heads of 64: 1880 118 and 116, 3920 101 and 91; 640 30 and 33.5.
+constexpr long long PAIR_ITEMS = 1024;
 // Columns of a key head from which the many-row kernel takes a slot, and the
 // least workgroups it takes: with fewer its serial pass over the blocks is the
 // longer one. 64 wide, 20 heads, us here and on attend_kernel: 320 workgroups
 // 47 and 37, 500 57 and 68, 2000 120 and 165; 128 wide: 256 54 and 53, 392 92
 // and 102, 1568 186 and 235. (The same form for a paged cache, codes widened
 // into shared memory, was no shorter than attend_kernel: 1564 rows after 1000
-// tokens 102 and 71.)
+// tokens 102 and 65.)
 constexpr long long MANY_COLUMNS = 64, MANY_ITEMS = 384;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
@@ -864,6 +899,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     const auto tiles = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 15) / 16; };
     const auto blocks = [](const AttendSeq& q) { return (q.len + BLOCK_TOKENS - 1) / BLOCK_TOKENS; };
     a.aligned = a.hd % 4 == 0 && a.qs % 4 == 0 && (uintptr_t)a.q % 16 == 0;
+    a.aligned_out = a.hd % 4 == 0 && (uintptr_t)a.out % 16 == 0;
     // Slots that many columns ask, in launches of their own.
     std::vector<AttendSeq> few, many;
     const auto wide = [&](const AttendSeq& q) { return ((long long)q.rows * a.group + 63) / 64; };
@@ -942,6 +978,9 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
             while (items_of(a.chunk) > room || split * a.kv_heads > SPLIT_ITEMS)
                 a.chunk += (a.chunk / 8 + waves) / waves * waves;
         }
+        long long two = 0;
+        for (int i = 0; i < a.n; ++i) two += (tiles(a.s[i]) + 1) / 2;
+        const bool pairs = paged && !split && two * a.kv_heads >= PAIR_ITEMS && 5 * whole >= 9 * two;
         int items = 0, groups = 0, parts = 0;
         for (int i = 0; i < CALL_SEQS; ++i) {
             AttendSeq& q = a.s[i];
@@ -953,7 +992,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
             q.start = items;
             q.group = groups;
             q.part = parts;
-            items += (int)tiles(q) * q.chunks;
+            items += pairs ? (int)((tiles(q) + 1) / 2) : (int)tiles(q) * q.chunks;
             if (q.chunks > 1) {
                 groups += (int)tiles(q);
                 parts += (int)tiles(q) * q.chunks;
@@ -964,6 +1003,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
                                          : (waves == 4 ? attend_kernel<64, false, 4> : attend_kernel<64, false, 8>))
                                 : (paged ? (waves == 4 ? attend_kernel<128, true, 4> : attend_kernel<128, true, 8>)
                                          : (waves == 4 ? attend_kernel<128, false, 4> : attend_kernel<128, false, 8>));
+        if (pairs) kernel = hdp == 64 ? attend_kernel<64, true, 4, 2> : attend_kernel<128, true, 4, 2>;
         hipLaunchKernelGGL(kernel, grid, block, 0, s, a);
         TRIT_HIP(hipGetLastError());
     }
