@@ -45,3 +45,12 @@ def test_serving_calls_refuse_before_a_device_is_needed():
         assert b"paged cache" in lib.trit_hip_last_error()
     lib.trit_hip_paged_free(None)
     lib.trit_hip_cross_free(None)
+
+
+def test_states_past_64_bits_are_refused():
+    """Sizes whose bytes, counted in 64 bits, come out as few or none."""
+    lib, out = hip.lib(), C.c_void_p()
+    for shape in ((1, 1 << 15, 64, 1 << 20, 1 << 26), (1, 1 << 15, 64, 1 << 20, (1 << 26) - 63),
+                  (1 << 16, 65535, 128, 1 << 20, 1 << 26), (1 << 13, 1 << 13, 128, 1 << 13, 1 << 16)):
+        assert lib.trit_hip_cross_new(*shape, C.byref(out)) == -1
+        assert b"memory" in lib.trit_hip_last_error(), (shape, lib.trit_hip_last_error())

@@ -140,17 +140,21 @@ int trit_hip_cross_new(int layers, int kv_heads, int head_dim, int slots, int ma
         if (head_dim <= 0 || head_dim > 128) fail("cross attention: head_dim must be 1 to 128");
         if (kv_heads > 65535 || slots > (1 << 20) || layers > (1 << 16) || max_keys > (1 << 26))
             fail("cross attention: at most 65535 heads, 2^20 slots, 2^16 layers and 2^26 keys");
+        // (Within those the number of bytes may pass 64 bits.)
+        const int wide = head_dim <= 64 ? 64 : 128, most = (max_keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+        if ((double)layers * slots * kv_heads * most * (BLOCK_TOKENS * wide * 4.0) > 0x1p48)
+            fail("cross attention: states of more memory than a device holds");
         auto c = std::make_unique<TritHipCross>();
         c->device = device_id();
         c->layers = layers;
         c->kv_heads = kv_heads;
         c->hd = head_dim;
-        c->hdp = head_dim <= 64 ? 64 : 128;
+        c->hdp = wide;
         c->slots = slots;
         c->max_keys = max_keys;
-        c->blocks = (max_keys + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
-        c->keys.assign((size_t)layers * slots, -1);
+        c->blocks = most;
         c->states.alloc((size_t)layers * c->layer_values() * 2);
+        c->keys.assign((size_t)layers * slots, -1);
         c->scratch.make(c->hdp, c->enter(nullptr));
         *out = c.release();
         return 0;
