@@ -461,6 +461,25 @@ def test_refusals(gpu):
     assert c.attention(0, ids[:0], [], x[:0], 2).shape == (0, 128)
 
 
+def test_a_refused_attention_writes_nothing(gpu):
+    """More query rows than a call takes, in a sequence behind more than one launch holds."""
+    print("case refused attention", flush=True)
+    lens = [1] * 140 + [2001]
+    c, ids, _ = filled(1, 1, lens)
+    q = np.ones((sum(lens), 400), np.float32)
+    D = Device()
+    try:
+        dq, out = D.upload(q), D.upload(np.full_like(q, 7.0))
+        with pytest.raises(hip.TritError, match="rows"):
+            c.attention_device(0, ids, lens, dq, 400, 400, out)
+        assert (D.download(out, q.shape) == 7.0).all()
+        c.attention_device(0, ids, lens[:140] + [2000], dq, 400, 400, out)
+        got = D.download(out, q.shape)
+        assert (got[:2140] != 7.0).all() and (got[2140] == 7.0).all()
+    finally:
+        D.free()
+
+
 def test_capture_is_refused(gpu):
     print("case capture", flush=True)
     import torch

@@ -906,6 +906,7 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
     long long wides = 0;
     for (const AttendSeq& q : seqs) {
         if (!q.rows) continue;
+        if (tiles(q) > MOST_TILES) fail("attention: more query rows than one launch takes");
         const bool is = !paged && (long long)q.rows * a.group >= MANY_COLUMNS;
         if (is) wides += wide(q);
         (is ? many : few).push_back(q);
@@ -920,7 +921,6 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
         long long items = 0;
         for (a.n = 0; at < many.size() && a.n < CALL_SEQS; ++at) {
             AttendSeq q = many[at];
-            if (wide(q) > MOST_TILES) fail("attention: more query rows than one launch takes");
             if (a.n && items + wide(q) > MOST_TILES) break;
             q.start = (int)items;
             items += wide(q);
@@ -937,7 +937,6 @@ void attend(AttendArgs& a, const std::vector<AttendSeq>& seqs, bool paged, Atten
         int most = 0;
         size_t to = from;
         for (a.n = 0; to < few.size() && a.n < CALL_SEQS; ++to) {
-            if (tiles(few[to]) > MOST_TILES) fail("attention: more query rows than one launch takes");
             if (a.n && whole + tiles(few[to]) > MOST_TILES) break;
             whole += tiles(few[to]);
             work += tiles(few[to]) * blocks(few[to]);
