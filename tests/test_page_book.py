@@ -259,3 +259,11 @@ def test_refusals_change_nothing(shim):
     x.append(1, [p], [[8]])
     x.fork([p])
     x.check()
+
+
+def test_a_negative_number_of_sequences_is_refused(shim):
+    x = Played(shim, 1, 4, 3)
+    a, b = x.open_new(2)
+    scratch = ints([0] * 64)
+    x.refused(shim.book_reorder(x.h, ints([a]), ints([b]), -1, scratch), "negative")
+    x.refused(shim.book_fork(x.h, ints([a]), -1, scratch, scratch), "negative")

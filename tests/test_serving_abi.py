@@ -2,6 +2,9 @@
 
 import ctypes as C
 
+import numpy as np
+import pytest
+
 from trit_amd import hip
 
 
@@ -54,3 +57,23 @@ def test_states_past_64_bits_are_refused():
                   (1 << 16, 65535, 128, 1 << 20, 1 << 26), (1 << 13, 1 << 13, 128, 1 << 13, 1 << 16)):
         assert lib.trit_hip_cross_new(*shape, C.byref(out)) == -1
         assert b"memory" in lib.trit_hip_last_error(), (shape, lib.trit_hip_last_error())
+
+
+def test_ids_and_counts_are_32_bit_integers():
+    """A value that 32 bits would change names no other sequence."""
+    for values in ([1 << 31], [-(1 << 31) - 1], np.array([1 << 32]), np.array([3], np.uint64) << 40, [0.5], [1.0],
+                   [True], ["1"], [None]):
+        with pytest.raises(hip.TritError, match="integers"):
+            hip._ids(values)
+    for values in ([], np.zeros(0), [3, 1], (3, 1), np.array([3, 1]), np.array([[3], [1]], np.uint8),
+                   np.array([3, 9, 1], np.int32)[::2]):
+        got = hip._ids(values)
+        assert got.dtype == np.int32 and got.flags.c_contiguous and got.tolist() in ([], [3, 1])
+
+
+def test_no_copy_into_a_freed_cache():
+    """A freed cache is not taken for the cache's own (NULL)."""
+    a, b = (hip.PagedCache.__new__(hip.PagedCache) for _ in range(2))
+    a.h = b.h = None
+    with pytest.raises(hip.TritError, match="freed"):
+        a.copy([0], into=b)

@@ -84,6 +84,7 @@ class PageBook {
     // Sequence ids[i] goes on with what parents[i] held before the call. A
     // parent's row goes to one of its children; only the others are copied.
     std::vector<RowCopy> reorder(const int* ids, const int* parents, int n) {
+        if (n < 0) refuse("a negative number of sequences");
         std::vector<int> at((size_t)sequences(), -1);  // id -> its place in the call
         for (int i = 0; i < n; ++i) {
             even(ids[i]);

@@ -747,7 +747,10 @@ def _ids(values):
     """Sequence ids, slots or row counts as the C calls read them (an int32 array as it is)."""
     if isinstance(values, np.ndarray) and values.dtype == np.int32 and values.flags.c_contiguous and values.ndim == 1:
         return values
-    return np.ascontiguousarray(np.asarray(values, dtype=np.int32).reshape(-1))
+    values = np.asarray(values).reshape(-1)
+    if values.size and (values.dtype.kind not in "iu" or int(values.min()) < -2**31 or int(values.max()) >= 2**31):
+        raise TritError("ids and counts must be integers of 32 bits")
+    return np.ascontiguousarray(values, np.int32)
 
 
 _CHAR, _ADDRESS = C.c_char.from_buffer, C.addressof
@@ -803,6 +806,8 @@ class PagedCache:
 
     def copy(self, sequences, into=None, stream=None):
         ids = _ids(sequences)
+        if into is not None and not into.h:
+            raise TritError("paged copy: the cache to copy into is freed")
         out = np.empty(ids.size, np.int32)
         check(lib().trit_hip_paged_copy(self.h, _at(ids), ids.size, into.h if into is not None else None, ptr(out),
                                         stream))
