@@ -20,6 +20,9 @@ constexpr int MOST_CHUNKS = 128;
 // The largest fixed-point value of three int8 digits, and the factor that
 // keeps the low part of an f16 pair clear of subnormal f16.
 constexpr float FIXED = 8323072.0f;  // 127 * 65536
+// What a product of the lowest digits starts from: its bits are a float's with
+// the product added, so that it needs no conversion.
+constexpr float LOWEST = 12582912.0f;  // 1.5 * 2^23
 constexpr float PAIR = 1024.0f, LOG_PAIR = 10.0f;
 // How far (in powers of two) scores may pass a softmax's reference: p * PAIR stays within f16.
 constexpr float SLACK = 5.0f;
@@ -51,6 +54,7 @@ template <int HDP>
 struct Running {
     float m = -INFINITY;  // the sums' reference, in powers of two: the largest score so far but for SLACK
     float l = 0.0f;       // this lane's part of the sum of 2^(score - m)
+    float extra = 0.0f;   // what each of acc holds too much
     v4f acc[HDP / 16];
 
     __device__ __forceinline__ void clear() {
@@ -59,7 +63,7 @@ struct Running {
     }
 };
 
-// Scores u * f (f >= 0 or NaN) of a block to probabilities of that block
+// Scores (u - off) * f (f >= 0 or NaN) of a block to probabilities of that block
 // alone, p = 2^((u - max) f) <= 1, in place; then the running sums take the
 // block's largest score as theirs. Returned: what scales the block's products
 // (0 where the column sees none of it). A block's probabilities become
@@ -68,7 +72,8 @@ struct Running {
 // (the same for the wave): `seen` of the block's tokens count, whatever the
 // others hold.
 template <int HDP>
-__device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mask, int seen, Running<HDP>& run) {
+__device__ __forceinline__ float block_softmax(float (&u)[16], float off, float f, bool mask, int seen,
+                                               Running<HDP>& run) {
     const int lq = (threadIdx.x % WAVE) / 16;
     if (mask) {
 #pragma unroll
@@ -80,7 +85,7 @@ __device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mas
     for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i]);
     top = column_max(top);
     const bool any = top > -INFINITY;
-    const float mb = any ? top * f : -INFINITY;
+    const float mb = any ? (top - off) * f : -INFINITY;
     // The difference first: never above 0, whatever the scores' size.
 #pragma unroll
     for (int i = 0; i < 16; ++i) u[i] = __builtin_amdgcn_exp2f((u[i] - top) * f);
@@ -98,6 +103,7 @@ __device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mas
         const float before = mn == run.m ? 1.0f : __builtin_amdgcn_exp2f(run.m - mn);
         run.m = mn;
         run.l *= before;
+        run.extra *= before;
 #pragma unroll
         for (int n = 0; n < HDP / 16; ++n)
 #pragma unroll
@@ -201,6 +207,20 @@ __device__ __forceinline__ v4i load16(const uint8_t* wave, uint32_t lane) {
     return *(const TRIT_GLOBAL v4i*)((const TRIT_GLOBAL uint8_t*)wave + lane);
 }
 
+// The three digits' products as one number plus LOWEST. |c| <= 128 * 127 *
+// 128, so the lowest one's stays within LOWEST's exponent and the others' sum
+// within 32 bits. LOWEST is one and a half codes of the largest query value or
+// probability, so it costs a sum no digit that counts; scores lose it with
+// their largest, outputs at the end. (A conversion in its place: a prompt of
+// 1564 rows after 1000 tokens 65 us, so 63.4; four of 1564 118, so 115.)
+__device__ __forceinline__ float join_digits(int c0, int c1, int c2) {
+    return __builtin_fmaf((float)((c2 << 8) + c1), 256.0f, __int_as_float(c0));
+}
+__device__ __forceinline__ v4i lowest() {
+    const int x = __float_as_int(LOWEST);
+    return v4i{x, x, x, x};
+}
+
 // A full block of int8 codes, its keys' and values' fragments in registers.
 // Both products run in integers: the query and the probabilities are three
 // int8 digits each, so their products with the codes are exact, and what is
@@ -213,15 +233,13 @@ __device__ __forceinline__ void codes_scores(const v4i (&kf)[HDP / 16], const v4
         v4i c[3];
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
-            c[j] = v4i{0, 0, 0, 0};
+            c[j] = j ? v4i{0, 0, 0, 0} : lowest();
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 c[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t * KS + ks], qd[j][ks], c[j], 0, 0, 0);
         }
-        // |c| <= 128 * 127 * 128: c1 * 256 + c0 stays within 32 bits.
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            u[4 * t + r] = __builtin_fmaf((float)c[2][r], 65536.0f, (float)((c[1][r] << 8) + c[0][r]));
+        for (int r = 0; r < 4; ++r) u[4 * t + r] = join_digits(c[0][r], c[1][r], c[2][r]);
         pin(u[4 * t], u[4 * t + 1], u[4 * t + 2], u[4 * t + 3]);
     }
 }
@@ -246,14 +264,13 @@ __device__ __forceinline__ void codes_values(const v4i (&vf)[HDP / 16], const fl
         v4i c[3];
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            c[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[n], pd[j], v4i{0, 0, 0, 0}, 0, 0, 0);
+            c[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[n], pd[j], j ? v4i{0, 0, 0, 0} : lowest(), 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float o = __builtin_fmaf((float)c[2][r], 65536.0f, (float)((c[1][r] << 8) + c[0][r]));
-            run.acc[n][r] = __builtin_fmaf(o, w, run.acc[n][r]);
-        }
+        for (int r = 0; r < 4; ++r)
+            run.acc[n][r] = __builtin_fmaf(join_digits(c[0][r], c[1][r], c[2][r]), w, run.acc[n][r]);
         pin(run.acc[n]);
     }
+    run.extra = __builtin_fmaf(LOWEST, w, run.extra);
 }
 
 __device__ __forceinline__ bool any_nan(v8h x) {
@@ -493,7 +510,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
                 for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024, lane16);
             }
             const float now =
-                block_softmax<HDP>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > least, seen - b * BLOCK_TOKENS, run);
+                block_softmax<HDP>(u, LOWEST, step * s0.x, (b + 1) * BLOCK_TOKENS > least, seen - b * BLOCK_TOKENS, run);
             // A column that sees nothing of the block takes nothing of it, also where its scale is NaN.
             codes_values<HDP>(vf, u, now == 0.0f && seen <= b * BLOCK_TOKENS ? 0.0f : now * s0.y * (1.0f / FIXED), run);
             if (more) {
@@ -514,7 +531,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) v16[i] = load8h(open + BLOCK / 2 + i * 512, lane16);
-            const float now = block_softmax<HDP>(u, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
+            const float now = block_softmax<HDP>(u, 0.0f, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
             open_values<HDP>(v16, u, now, tokens, sees, run);
         }
     } else {
@@ -543,7 +560,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             const bool more = b + KEYED < end;
             if (more && AHEAD) load(kf, b + KEYED, 0);
             const float now =
-                block_softmax<HDP>(u, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
+                block_softmax<HDP>(u, 0.0f, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
             f16_values<HDP>(vf, u, now, run);
             if (more && !AHEAD) load(kf, b + KEYED, 0);
             if (more && AHEAD) load(vf, b + KEYED, 1);
@@ -556,7 +573,8 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     }
     if (col < own) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) *(v4f*)(part[w][col] + 16 * n + 4 * lq) = run.acc[n];
+        for (int n = 0; n < NT; ++n)
+            *(v4f*)(part[w][col] + 16 * n + 4 * lq) = PAGED ? run.acc[n] - run.extra : run.acc[n];
     }
     __syncthreads();
     // Four dims of a column: the sums of the waves' parts, relative to their largest score m.
