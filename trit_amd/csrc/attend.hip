@@ -35,15 +35,15 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // The three digits of 4 fixed-point values (|x| <= FIXED), each digit's 4
-// bytes in a word: x + 0x808080 carries what a signed digit takes from the
-// next one, and flipping the top bits makes the bytes signed.
-__device__ __forceinline__ void digits4(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, int& d0, int& d1, int& d2) {
-    const uint32_t t0 = (x0 + 0x808080u) ^ 0x808080u, t1 = (x1 + 0x808080u) ^ 0x808080u;
-    const uint32_t t2 = (x2 + 0x808080u) ^ 0x808080u, t3 = (x3 + 0x808080u) ^ 0x808080u;
-    const uint32_t a = __builtin_amdgcn_perm(t1, t0, 0x05010400u), b = __builtin_amdgcn_perm(t3, t2, 0x05010400u);
-    d0 = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
-    d1 = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
-    const uint32_t c = __builtin_amdgcn_perm(t1, t0, 0x0c0c0602u), d = __builtin_amdgcn_perm(t3, t2, 0x0c0c0602u);
+// bytes in a word; the values come with CARRY added, which carries what a
+// signed low digit takes from the next one. Flipping the low digits' top bits
+// makes them signed; the highest one is.
+constexpr int CARRY = 0x8080;
+__device__ __forceinline__ void digits4(const uint32_t (&x)[4], int& d0, int& d1, int& d2) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    d0 = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+    d1 = (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
+    const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0602u), d = __builtin_amdgcn_perm(x[3], x[2], 0x0c0c0602u);
     d2 = (int)__builtin_amdgcn_perm(d, c, 0x05040100u);
 }
 
@@ -171,9 +171,9 @@ __device__ __forceinline__ void put_queries(const float (&v)[HDP / 16], Queries<
         for (int i = 0; i < E; i += 4) {
             uint32_t x[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = finite ? (uint32_t)(int)__builtin_rintf(v[i + r] * inv) : 0u;
+            for (int r = 0; r < 4; ++r) x[r] = (uint32_t)((finite ? (int)__builtin_rintf(v[i + r] * inv) : 0) + CARRY);
             int d[3];
-            digits4(x[0], x[1], x[2], x[3], d[0], d[1], d[2]);
+            digits4(x, d[0], d[1], d[2]);
             const int e = e0 + i, at = e / 64 * 1024 + (e % 64 / 16 * 16 + col) * 16 + e % 16;
 #pragma unroll
             for (int j = 0; j < 3; ++j) *(int*)(out.digits[j] + at) = d[j];
@@ -250,11 +250,11 @@ __device__ __forceinline__ void codes_values(const v4i (&vf)[HDP / 16], const fl
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         uint32_t x[4];
-        // round(p * FIXED) in the low bits of a float of exponent 2^23.
+        // round(p * FIXED) + CARRY in the low bits of a float of exponent 2^23: below 2^23 as p is at most 1.
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = __float_as_uint(__builtin_fmaf(p[4 * t + r], FIXED, 8388608.0f));
+        for (int r = 0; r < 4; ++r) x[r] = __float_as_uint(__builtin_fmaf(p[4 * t + r], FIXED, 8388608.0f + CARRY));
         int d0, d1, d2;
-        digits4(x[0], x[1], x[2], x[3], d0, d1, d2);
+        digits4(x, d0, d1, d2);
         pd[0][t] = d0;
         pd[1][t] = d1;
         pd[2][t] = d2;
