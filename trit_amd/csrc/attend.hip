@@ -63,17 +63,16 @@ struct Running {
     }
 };
 
-// Scores (u - off) * f (f >= 0 or NaN) of a block to probabilities of that block
-// alone, p = 2^((u - max) f) <= 1, in place; then the running sums take the
-// block's largest score as theirs. Returned: what scales the block's products
-// (0 where the column sees none of it). A block's probabilities become
-// fixed-point values or f16 pairs relative to its own maximum, so that a long
-// tail of small ones next to one large one far away keeps its digits. mask
-// (the same for the wave): `seen` of the block's tokens count, whatever the
-// others hold.
-template <int HDP>
-__device__ __forceinline__ float block_softmax(float (&u)[16], float off, float f, bool mask, int seen,
-                                               Running<HDP>& run) {
+// Scores u * f (f >= 0 or NaN; of codes: (u - LOWEST) * f) of a block to
+// probabilities of that block alone, p = 2^((u - max) f) <= 1, in place; then
+// the running sums take the block's largest score as theirs. Returned: what
+// scales the block's products (0 where the column sees none of it). A block's
+// probabilities become fixed-point values or f16 pairs relative to its own
+// maximum, so that a long tail of small ones next to one large one far away
+// keeps its digits. mask (the same for the wave): `seen` of the block's tokens
+// count, whatever the others hold.
+template <int HDP, bool CODES>
+__device__ __forceinline__ float block_softmax(float (&u)[16], float f, bool mask, int seen, Running<HDP>& run) {
     const int lq = (threadIdx.x % WAVE) / 16;
     if (mask) {
 #pragma unroll
@@ -85,10 +84,17 @@ __device__ __forceinline__ float block_softmax(float (&u)[16], float off, float 
     for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, u[i]);
     top = column_max(top);
     const bool any = top > -INFINITY;
-    const float mb = any ? (top - off) * f : -INFINITY;
-    // The difference first: never above 0, whatever the scores' size.
+    const float scaled = top * f;
+    const float mb = !any ? -INFINITY : CODES ? __builtin_fmaf(-LOWEST, f, scaled) : scaled;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) u[i] = __builtin_amdgcn_exp2f((u[i] - top) * f);
+    for (int i = 0; i < 16; ++i) {
+        // Codes: what the rounding of the largest score lifts above 1 is 1, as digits need it. A NaN becomes 0, but
+        // then f is NaN and with it what is returned. f16: the difference first, never above 0.
+        if (CODES)
+            u[i] = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(__builtin_fmaf(u[i], f, -scaled)), 0.0f, 1.0f);
+        else
+            u[i] = __builtin_amdgcn_exp2f((u[i] - top) * f);
+    }
     if (mask) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -510,7 +516,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
                 for (int i = 0; i < NT; ++i) kf[i] = load16(next + i * 1024, lane16);
             }
             const float now =
-                block_softmax<HDP>(u, LOWEST, step * s0.x, (b + 1) * BLOCK_TOKENS > least, seen - b * BLOCK_TOKENS, run);
+                block_softmax<HDP, true>(u, step * s0.x, (b + 1) * BLOCK_TOKENS > least, seen - b * BLOCK_TOKENS, run);
             // A column that sees nothing of the block takes nothing of it, also where its scale is NaN.
             codes_values<HDP>(vf, u, now == 0.0f && seen <= b * BLOCK_TOKENS ? 0.0f : now * s0.y * (1.0f / FIXED), run);
             if (more) {
@@ -531,7 +537,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) v16[i] = load8h(open + BLOCK / 2 + i * 512, lane16);
-            const float now = block_softmax<HDP>(u, 0.0f, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
+            const float now = block_softmax<HDP, false>(u, qs.top[col] * (LOG2E / PAIR), true, min(sees, tokens), run);
             open_values<HDP>(v16, u, now, tokens, sees, run);
         }
     } else {
@@ -560,7 +566,7 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
             const bool more = b + KEYED < end;
             if (more && AHEAD) load(kf, b + KEYED, 0);
             const float now =
-                block_softmax<HDP>(u, 0.0f, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
+                block_softmax<HDP, false>(u, step, (b + 1) * BLOCK_TOKENS > seen, seen - b * BLOCK_TOKENS, run);
             f16_values<HDP>(vf, u, now, run);
             if (more && !AHEAD) load(kf, b + KEYED, 0);
             if (more && AHEAD) load(vf, b + KEYED, 1);
