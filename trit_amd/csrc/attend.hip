@@ -157,7 +157,7 @@ __device__ __forceinline__ void load_queries(const float* q, bool valid, bool al
     for (int i = 0; i < E; ++i) v[i] = valid && e0 + i < hd ? v[i] * scale : 0.0f;
 }
 template <int HDP, bool DIGITS>
-__device__ __forceinline__ void put_queries(const float (&v)[HDP / 16], Queries<HDP, DIGITS>& out) {
+__device__ __forceinline__ void put_queries(const float (&v)[HDP / 16], bool pairs, Queries<HDP, DIGITS>& out) {
     constexpr int E = HDP / 16;
     const int col = threadIdx.x / 16, e0 = threadIdx.x % 16 * E;
     float top = 0.0f;
@@ -185,6 +185,7 @@ __device__ __forceinline__ void put_queries(const float (&v)[HDP / 16], Queries<
             for (int j = 0; j < 3; ++j) *(int*)(out.digits[j] + at) = d[j];
         }
     }
+    if (!pairs) return;
     const float inv = PAIR / top;
 #pragma unroll
     for (int i = 0; i < E; i += 4) {
@@ -457,19 +458,23 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
                                      a.aligned, a.hd, a.scale, qv[i]);
         }
     }
-    auto put_all = [&] {
-        if (t < 256) {
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) put_queries<HDP, PAGED>(qv[i], queries[i]);
-        }
-        __syncthreads();
-    };
     // Keys the lane's column sees, and the wave's tile's most and least.
     const int ahead = PAGED ? seq.len - seq.rows + 1 + row0 : seq.len;
     const int least = PAGED ? ahead + (rest + 16 * mine) / a.group : ahead;
     const int most = own <= 0 ? 0 : PAGED ? ahead + (rest + 16 * mine + own - 1) / a.group : ahead;
     const int seen = PAGED ? ahead + row_of(16 * mine + min(col, max(own - 1, 0))) : ahead;
     const int b0 = chunk * a.chunk;
+    // Whether any column of the workgroup meets f16 values.
+    const int full = seq.len / BLOCK_TOKENS;  // full blocks hold codes
+    const bool pairs =
+        !PAGED || (full < b0 + a.chunk && ahead + (rest + cols - 1) / a.group > full * BLOCK_TOKENS);
+    auto put_all = [&] {
+        if (t < 256) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) put_queries<HDP, PAGED>(qv[i], pairs, queries[i]);
+        }
+        __syncthreads();
+    };
     const int all = (most + BLOCK_TOKENS - 1) / BLOCK_TOKENS, end = all < b0 + a.chunk ? all : b0 + a.chunk;
 
     Running<HDP> run;
@@ -477,7 +482,6 @@ __global__ __launch_bounds__(WAVES* WAVE, 2) void attend_kernel(AttendArgs a) {
     int b = b0 + turn;
     const uint32_t lane16 = lane * 16;
     if constexpr (PAGED) {
-        const int full = seq.len / BLOCK_TOKENS;  // full blocks hold codes
         const int last = end < full ? end : full;
         const int* table = a.table + (size_t)seq.place * a.table_stride;
         v4i kf[NT], vf[NT];
@@ -890,13 +894,14 @@ constexpr long long SPLIT_ITEMS = 1024;
 // Workgroups of 8 waves that the compute units take at once.
 constexpr long long FEW_ITEMS = 256;
 // The least workgroups of two tiles that a paged launch takes, where nine
-// tenths of the second ones are there (60 requests of a single tile 29 us with
-// one, 36 with room for two): a wave's keys are twice as many, so its fixed
-// part (queries, first loads, join) weighs half. 16/8 heads of 128, us with
-// one tile and with two: 3000 rows after 1000 tokens (1500 such workgroups)
-// 149 and 141, two prompts of 1564 (1568) 73 and 63, four (3136) 135 and 119;
-// 1564 rows after 1000 (784) 65.5 and 64.5, 1024 after 1024 (512) 38 and 39.
-// 20 heads of 64: 1880 118 and 116, 3920 101 and 91; 640 30 and 33.5.
+// tenths of the second ones are there (60 requests of a single tile, 20 heads
+// of 64, 29 us with one, 34 with room for two): a wave's keys are twice as
+// many, so its fixed part (queries, first loads, join) weighs half. 16/8 heads
+// of 128, us with one tile and with two: 3000 rows after 1000 tokens (1500 such
+// workgroups) 137 and 129, two prompts of 1564 (1568) 66 and 59, four (3136)
+// 126 and 111; 1564 rows after 1000 (784) 60.3 and 60.9, 512 after 512 (256)
+// 13.2 and 18.3. 20 heads of 64: 1880 103 and 101, 3920 90 and 80; 640 27 and
+// 30.
 constexpr long long PAIR_ITEMS = 1024;
 // Columns of a key head from which the many-row kernel takes a slot, and the
 // least workgroups it takes: with fewer its serial pass over the blocks is the
@@ -904,7 +909,7 @@ constexpr long long PAIR_ITEMS = 1024;
 // 47 and 37, 500 57 and 68, 2000 120 and 165; 128 wide: 256 54 and 53, 392 92
 // and 102, 1568 186 and 235. (The same form for a paged cache, codes widened
 // into shared memory, was no shorter than attend_kernel: 1564 rows after 1000
-// tokens 102 and 65.)
+// tokens 102 and 61.)
 constexpr long long MANY_COLUMNS = 64, MANY_ITEMS = 384;
 
 void AttendScratch::make(int hdp, hipStream_t s) {
